@@ -474,6 +474,66 @@ ORNITH_MOE_B200_EXPORT cudaError_t ornith_head_i8_tile_launch(
 /* Replaces ornith_head_i8_tile_shortlist (head_i8_tile_consumer.cpp:293): 1. */
 ORNITH_MOE_B200_EXPORT int ornith_head_i8_tile_shortlist(void);
 
+/* ------------------------------------------------------------------------
+ * Matrix-vector products with 4-bit weights in the ordinary checkpoint form
+ * (group scales, integer zero points, activations as they are).  No
+ * counterpart in the reference, whose 4-bit layers are the G256 banks above:
+ *   out[m][n] = sum_g s[n][g] * sum_{k in g} x[m][k] * (c[n][k] - z[n][g])
+ * Shapes: 0 <= M <= 16; 1 <= N <= 2^22; group 32, 64, 128 or 256; K a multiple
+ * of group, at most 16384.  Types: 0 bf16, 1 fp16, 2 fp32 (out only).
+ * Sums in fp32, one rounding to the output's type.  Flags (sticky, the dense
+ * library's bits): 4 non-finite fp32 result, 8 non-finite stored 16-bit value.
+ * ------------------------------------------------------------------------ */
+
+/* Lays a weight out for ornith_moe_b200_w4_launch, once: codes UINT32[N][K/8]
+ * (value 8j + d of a row in bits 4d of its word j), scales 16-bit [N][K/group],
+ * zeros uint8 [N][K/group] in 0..15 (only the low four bits are used) or null for 8 ->
+ * tiles UINT32[ceil(N/16)][ceil(K/64)][32][4], tile_scales
+ * UINT32[ceil(N/16)][K/group][8], tile_zeros uint8 [ceil(N/16)][K/group][8]
+ * (null iff zeros is).  Buffers must not overlap.  Alignment: tiles 16 B, codes
+ * and tile_scales 4 B, scales 2 B. */
+ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_w4_pack(
+    const void* codes, const void* scales_16, const void* zeros_u8, void* tiles, void* tile_scales,
+    void* tile_zeros, int N, int K, int group, cudaStream_t stream);
+
+/* x [M][K] with x_stride values between rows (at least K, a multiple of 8;
+ * unused for one row) -> out [M][N] of x_type or fp32.  scale_type is the type
+ * of the packed scales, tile_zeros null for zero points of 8.  M == 0 returns
+ * success without touching a pointer.  No workspace.  Alignment: x and tiles
+ * 16 B, tile_scales and flags 4 B, out its type's; out and flags overlap
+ * nothing. */
+ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_w4_launch(
+    const void* x, int64_t x_stride, int x_type, const void* tiles, const void* tile_scales, int scale_type,
+    const void* tile_zeros, void* out, int out_type, void* flags, int M, int N, int K, int group,
+    cudaStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Token sampling, the step after the head.  No counterpart in the reference,
+ * which leaves it to vLLM.  Per row of logits x[0..vocab), with
+ * w_i = exp((x_i - max x) / temperature):
+ *   A = tokens with w_i >= min_p;  K = the first top_k of A by (x descending,
+ *   index ascending);  P = the smallest prefix of K, in that order, with mass
+ *   >= top_p * mass(K), one token at least;  token = the first i, in index
+ *   order, with sum_{j <= i, j in P} w_j > uniform * mass(P).
+ * temperature 0: the largest logit, lowest index.  top_k < 1 or >= vocab,
+ * top_p >= 1 and min_p 0 switch their cut off.  logprobs: the model's own
+ * x_token - max x - log sum_i exp(x_i - max x).  Weights and their sums are
+ * 64-bit fixed point: the token does not depend on the order of summation.
+ * -inf logits are never drawn.  A row that cannot be sampled gets token -1 and
+ * log probability NaN and raises (sticky) 1: NaN or +inf among its logits,
+ * 2: a parameter out of range (temperature outside [0, 1e30], top_p negative,
+ * min_p outside [0, 1], uniform outside [0, 1), any NaN), 4: every logit -inf.
+ * 0 <= M, 1 <= vocab <= 524288; type 0 bf16, 1 fp16, 2 fp32; stride: values
+ * between rows, at least vocab (unused for one row); any alignment of the
+ * type.  temperature, top_p, min_p, uniform fp32 [M], top_k int32 [M]; all but
+ * uniform may be null (temperature 1, no cut).  tokens int32 [M], logprobs fp32
+ * [M] or null.  tokens, logprobs and flags overlap nothing.  No workspace.
+ * ------------------------------------------------------------------------ */
+ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_sample_launch(
+    const void* logits, int64_t stride, int type, const void* temperature_f32, const void* top_k_i32,
+    const void* top_p_f32, const void* min_p_f32, const void* uniform_f32, void* tokens_i32, void* logprobs_f32,
+    void* flags_u32, int M, int vocab, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,7 +16,7 @@ LIB = HERE / 'libornith_moe_b200.so'
 DEBUG_LIB = HERE / 'libornith_moe_b200_debug.so'
 DEBUG_FLAGS = ('-DORNITH_DEBUG_BOUNDS=1',)
 SOURCES = ['moe_api.cu', 'moe_generic.cu', 'moe_decode.cu', 'moe_decode1.cu', 'moe_prefill.cu', 'moe_noalloc.cu', 'dense_g256.cu', 'head_i8.cu',
-           'ep_plan.cu', 'ep_p2p.cu']
+           'ep_plan.cu', 'ep_p2p.cu', 'w4_matvec.cu', 'sample.cu']
 NVCC = os.environ.get('NVCC', '/usr/local/cuda/bin/nvcc')
 FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', '-std=c++17',
          '-fmad=false', '-Xcompiler', '-fPIC,-fvisibility=hidden', '-shared', '-rdc=false',

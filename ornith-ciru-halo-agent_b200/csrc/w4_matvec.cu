@@ -1,0 +1,376 @@
+// Matrix-vector products of 1 to 16 rows with 4-bit weights and group scales:
+//
+//   out[m][n] = sum_g s[n][g] * sum_{k in group g} x[m][k] * (c[n][k] - z[n][g])
+//
+// codes c and zero points z in 0..15 (z = 8 without zero points), bf16 or fp16
+// activations as they are, groups of 32, 64, 128 or 256 values of K.  It stands
+// beside the G256 projections for checkpoints in the ordinary 4-bit form (no
+// Hadamard rotation, no quantised activations).
+//
+// Arithmetic.  c - z is an integer of at most 4 bits and a sign, exact in bf16
+// and fp16, so every product x * (c - z) is exact in fp32.  Runs of 32 or 64
+// products (never across a group) are summed in the tensor core's fp32
+// accumulator; each run is scaled and added to the row's fp32 sum with one FMA;
+// the only rounding below fp32 is the store in the output's type.
+//
+// Layout.  A tile is 16 rows of N times 64 values of K = 512 bytes, lane
+// l = 4r + t holding 16 of them as four words, one per mma.m16n8k16 step, in
+// that instruction's A-fragment order: word w of lane (r, t) covers rows r and
+// r + 8 and k = 64c + 32(w / 2) + 8t + 4(w % 2) + {0..3}.  Bits 4j of the two
+// half words hold the two values of fragment register j, so (word >> 4j) &
+// 0x000f000f is the register up to an exponent.  The order of k inside a step
+// is free as long as both operands agree; this one keeps every step inside 32
+// consecutive values (the smallest group) and makes a lane's activations for
+// two steps 16 consecutive bytes of x.
+//
+// What bounds it: the stream of the codes, N*K/2 bytes.  One warp reads a tile
+// with one 16-byte load per lane, four tiles ahead in registers.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "../../include/ornith_moe_b200.h"
+#include "abi_check.h"
+#include "nvtx_range.h"
+
+namespace ornith {
+void count_launches(int n);
+
+namespace w4 {
+
+constexpr int kMaxM = 16, kWarps = 8, kMaxK = 16384, kMaxN = 1 << 22, kSms = 148;
+constexpr uint32_t kFlagProjection = 4, kFlagStored = 8;  // the dense library's bits
+
+bool shape_ok(int N, int K, int group) {
+    return N > 0 && N <= kMaxN && K > 0 && K <= kMaxK && (group == 32 || group == 64 || group == 128 || group == 256) &&
+           K % group == 0;
+}
+inline int row_tiles(int N) { return (N + 15) / 16; }
+inline int k_chunks(int K) { return (K + 63) / 64; }
+
+// ---------------------------------------------------------------------------
+// layout, once per weight
+// ---------------------------------------------------------------------------
+
+// One thread per word of a tile; codes U32[N][K/8], value 8j + d of a row in
+// bits 4d of word j.  Rows past N and values past K are code 0: the first are
+// not stored, the second never enter a product (see the half-chunk test).
+__global__ __launch_bounds__(256) void w4_pack_codes_kernel(const uint32_t* codes, uint32_t* tiles, int N, int K,
+                                                            size_t words) {
+    const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= words) return;
+    const int chunks = (K + 63) / 64;
+    const int w = int(i & 3), lane = int((i >> 2) & 31), r = lane >> 2, t = lane & 3;
+    const size_t tile = i >> 7;
+    const int c = int(tile % chunks), row = int(tile / chunks) * 16 + r;
+    const int k = 64 * c + 32 * (w >> 1) + 8 * t + 4 * (w & 1);
+    uint32_t four[2] = {0u, 0u};  // nibbles k..k+3 of rows r and r + 8
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (row + 8 * h < N && k < K)
+            four[h] = (codes[size_t(row + 8 * h) * (K / 8) + k / 8] >> (4 * (k & 7))) & 0xffffu;
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)  // e: low or high half of the register
+#pragma unroll
+        for (int p = 0; p < 2; ++p)  // p: first or second pair of k
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                word |= ((four[h] >> (4 * (2 * p + e))) & 15u) << (16 * e + 4 * (2 * p + h));
+    tiles[i] = word;
+}
+
+// Scales 16-bit [N][K/G] -> [row tile][group][r] pairs (row r, row r + 8);
+// zero points u8 likewise, the pair in one byte.
+__global__ __launch_bounds__(256) void w4_pack_meta_kernel(const uint16_t* scales, const uint8_t* zeros,
+                                                           uint32_t* tile_scales, uint8_t* tile_zeros, int N,
+                                                           int groups, size_t pairs) {
+    const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= pairs) return;
+    const int r = int(i & 7);
+    const size_t tg = i >> 3;
+    const int g = int(tg % groups), row = int(tg / groups) * 16 + r;
+    uint32_t s = 0, z = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (row + 8 * h < N) {
+            const size_t at = size_t(row + 8 * h) * groups + g;
+            s |= uint32_t(scales[at]) << (16 * h);
+            if (zeros) z |= (zeros[at] & 15u) << (4 * h);
+        }
+    tile_scales[i] = s;
+    if (zeros) tile_zeros[i] = uint8_t(z);
+}
+
+// ---------------------------------------------------------------------------
+// product
+// ---------------------------------------------------------------------------
+
+struct Args {
+    const void* x;
+    int64_t x_stride;  // values between rows of x
+    const uint4* tiles;
+    const uint32_t* scales;
+    const uint8_t* zeros;
+    void* out;
+    uint32_t* flags;
+    int M, N, K, chunks, groups, group_shift, split, out_f32, scale_f16;
+};
+
+template <bool F16>
+struct Num;
+template <>
+struct Num<false> {  // bf16: 128 + c has c in the low mantissa bits
+    static constexpr uint32_t kMagic = 0x43004300u;
+    static __device__ __forceinline__ uint32_t bias(uint32_t z) { return kMagic | z | z << 16; }
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <>
+struct Num<true> {  // fp16: 1024 + c
+    static constexpr uint32_t kMagic = 0x64006400u;
+    static __device__ __forceinline__ uint32_t bias(uint32_t z) { return kMagic | z | z << 16; }
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ float scale_value(uint32_t bits16, int f16) {
+    return f16 ? __half2float(__ushort_as_half(uint16_t(bits16))) : __uint_as_float(bits16 << 16);
+}
+
+// Streamed once: do not keep the codes in L1.
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+// kWarps warps; `split` warps (a power of two up to kWarps) share a row tile,
+// taking its chunks in turn, and join their sums through shared memory.
+// MT: tiles of 8 activation rows; FINE: groups of 32, two runs per chunk.
+template <bool F16, int MT, bool ZP, bool FINE>
+__global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
+    constexpr int kAhead = 4, kRuns = FINE ? 2 : 1;
+    __shared__ float joined[kWarps][16][8 * MT + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+    const int part = warp & (a.split - 1);
+    const int per_cta = kWarps / a.split;
+    const int row_tile = blockIdx.x * per_cta + warp / a.split;
+    const int n_tiles = (a.N + 15) / 16;
+    float acc[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+
+    if (row_tile < n_tiles) {
+        const uint4* tile = a.tiles + size_t(row_tile) * a.chunks * 32 + lane;
+        const uint32_t* scale = a.scales + size_t(row_tile) * a.groups * 8 + r;
+        const uint8_t* zero = ZP ? a.zeros + size_t(row_tile) * a.groups * 8 + r : nullptr;
+        const uint16_t* xrow[MT];
+        bool has[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            has[i] = 8 * i + r < a.M;
+            xrow[i] = static_cast<const uint16_t*>(a.x) + (has[i] ? (8 * i + r) * a.x_stride : 0) + 8 * t;
+        }
+        uint4 code[kAhead];
+        uint32_t sc[kAhead][kRuns], zp[kAhead][kRuns];
+        auto fetch = [&](int slot, int c) {
+            if (c >= a.chunks) return;
+            code[slot] = load_stream(tile + size_t(c) * 32);
+#pragma unroll
+            for (int h = 0; h < kRuns; ++h) {
+                // the last chunk of a K that is 32 more than a multiple of 64 has one group
+                const int g = min((64 * c + 32 * h) >> a.group_shift, a.groups - 1);
+                sc[slot][h] = __ldg(scale + g * 8);
+                zp[slot][h] = ZP ? uint32_t(__ldg(zero + g * 8)) : 0x88u;
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) fetch(d, part + d * a.split);
+        for (int base = part; base < a.chunks; base += kAhead * a.split) {
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) {
+                const int c = base + d * a.split;
+                if (c >= a.chunks) break;
+                const uint32_t word[4] = {code[d].x, code[d].y, code[d].z, code[d].w};
+                uint32_t s2[kRuns], z2[kRuns];
+#pragma unroll
+                for (int h = 0; h < kRuns; ++h) s2[h] = sc[d][h], z2[h] = zp[d][h];
+                fetch(d, c + kAhead * a.split);
+                float run[MT][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (FINE && 64 * c + 32 * h >= a.K) break;  // the same for the whole warp
+                    uint4 b[MT];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        b[i] = has[i] ? __ldg(reinterpret_cast<const uint4*>(xrow[i] + 64 * c + 32 * h))
+                                      : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t z = z2[FINE ? h : 0];
+                    const uint32_t bias_lo = Num<F16>::bias(z & 15u), bias_hi = Num<F16>::bias(z >> 4);
+                    if (h == 0 || FINE) {
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) run[i][j] = 0.f;
+                    }
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        uint32_t frag[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            frag[j] = Num<F16>::sub(((word[2 * h + p] >> (4 * j)) & 0x000f000fu) | Num<F16>::kMagic,
+                                                    j & 1 ? bias_hi : bias_lo);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+                            Num<F16>::mma(run[i], frag, p ? b[i].z : b[i].x, p ? b[i].w : b[i].y);
+                    }
+                    if (h == 1 || FINE) {
+                        const uint32_t s = s2[FINE ? h : 0];
+                        const float lo = scale_value(s & 0xffffu, a.scale_f16), hi = scale_value(s >> 16, a.scale_f16);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            acc[i][0] = __fmaf_rn(lo, run[i][0], acc[i][0]);
+                            acc[i][1] = __fmaf_rn(lo, run[i][1], acc[i][1]);
+                            acc[i][2] = __fmaf_rn(hi, run[i][2], acc[i][2]);
+                            acc[i][3] = __fmaf_rn(hi, run[i][3], acc[i][3]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) joined[warp][r + 8 * (j >> 1)][8 * i + 2 * t + (j & 1)] = acc[i][j];
+    __syncthreads();
+    uint32_t fault = 0;
+    const int rows = 16 * per_cta;  // rows of N of this CTA
+    for (int i = threadIdx.x; i < rows * a.M; i += kWarps * 32) {
+        const int m = i / rows, row = i % rows, n = blockIdx.x * rows + row;
+        if (n >= a.N) continue;
+        float v = 0.f;
+        for (int p = 0; p < a.split; ++p) v = __fadd_rn(v, joined[(row >> 4) * a.split + p][row & 15][m]);
+        if (!isfinite(v)) fault |= kFlagProjection;
+        const size_t at = size_t(m) * a.N + n;
+        if (a.out_f32) {
+            static_cast<float*>(a.out)[at] = v;
+        } else if (F16) {
+            const __half h = __float2half_rn(v);
+            if (!isfinite(__half2float(h))) fault |= kFlagStored;
+            static_cast<__half*>(a.out)[at] = h;
+        } else {
+            const __nv_bfloat16 h = __float2bfloat16_rn(v);
+            if (!isfinite(__bfloat162float(h))) fault |= kFlagStored;
+            static_cast<__nv_bfloat16*>(a.out)[at] = h;
+        }
+    }
+    if (fault) atomicOr(a.flags, fault);
+}
+
+template <bool F16, int MT>
+void launch(const Args& a, bool zp, bool fine, int blocks, cudaStream_t stream) {
+    auto* kernel = zp ? (fine ? w4_matvec_kernel<F16, MT, true, true> : w4_matvec_kernel<F16, MT, true, false>)
+                      : (fine ? w4_matvec_kernel<F16, MT, false, true> : w4_matvec_kernel<F16, MT, false, false>);
+    kernel<<<blocks, kWarps * 32, 0, stream>>>(a);
+}
+
+}  // namespace w4
+}  // namespace ornith
+
+using namespace ornith;
+
+extern "C" cudaError_t ornith_moe_b200_w4_pack(const void* codes, const void* scales, const void* zeros, void* tiles,
+                                               void* tile_scales, void* tile_zeros, int N, int K, int group,
+                                               cudaStream_t stream) {
+    using namespace w4;
+    if (!shape_ok(N, K, group) || (zeros == nullptr) != (tile_zeros == nullptr)) return cudaErrorInvalidValue;
+    const int groups = K / group;
+    const size_t words = size_t(row_tiles(N)) * k_chunks(K) * 128, pairs = size_t(row_tiles(N)) * groups * 8;
+    const void* const ptr[5] = {codes, scales, tiles, tile_scales, nullptr};
+    const size_t size[5] = {size_t(N) * K / 2, size_t(N) * groups * 2, words * 4, pairs * 4, 0};
+    const uintptr_t align[5] = {4, 2, 16, 4, 1};
+    if (!buffers_ok(ptr, size, align, 2, 4)) return cudaErrorInvalidValue;
+    if (zeros) {
+        const void* const zptr[6] = {codes, scales, zeros, tiles, tile_scales, tile_zeros};
+        const size_t zsize[6] = {size[0], size[1], size_t(N) * groups, size[2], size[3], pairs};
+        const uintptr_t zalign[6] = {4, 2, 1, 16, 4, 1};
+        if (!buffers_ok(zptr, zsize, zalign, 3)) return cudaErrorInvalidValue;
+    }
+    count_launches(2);
+    w4_pack_codes_kernel<<<unsigned((words + 255) / 256), 256, 0, stream>>>(static_cast<const uint32_t*>(codes),
+                                                                            static_cast<uint32_t*>(tiles), N, K, words);
+    cudaError_t st = cudaGetLastError();
+    if (st != cudaSuccess) return st;
+    w4_pack_meta_kernel<<<unsigned((pairs + 255) / 256), 256, 0, stream>>>(
+        static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), static_cast<uint32_t*>(tile_scales),
+        static_cast<uint8_t*>(tile_zeros), N, groups, pairs);
+    return cudaGetLastError();
+}
+
+extern "C" cudaError_t ornith_moe_b200_w4_launch(const void* x, int64_t x_stride, int x_type, const void* tiles,
+                                                 const void* tile_scales, int scale_type, const void* tile_zeros,
+                                                 void* out, int out_type, void* flags, int M, int N, int K, int group,
+                                                 cudaStream_t stream) {
+    using namespace w4;
+    if (!shape_ok(N, K, group) || M < 0 || M > kMaxM || x_type < 0 || x_type > 1 || scale_type < 0 || scale_type > 1 ||
+        (out_type != x_type && out_type != 2))
+        return cudaErrorInvalidValue;
+    if (M == 0) return cudaSuccess;
+    // every row of x starts on 16 bytes and rows do not overlap; the stride of a single row is not used
+    if (x_stride < K || x_stride % 8 || x_stride > (int64_t(1) << 40)) {
+        if (M != 1) return cudaErrorInvalidValue;
+        x_stride = 0;
+    }
+    const int groups = K / group;
+    const size_t pairs = size_t(row_tiles(N)) * groups * 8;
+    const void* const ptr[6] = {x, tiles, tile_scales, tile_zeros, out, flags};
+    const size_t size[6] = {(size_t(M - 1) * size_t(x_stride) + size_t(K)) * 2, size_t(row_tiles(N)) * k_chunks(K) * 512,
+                            pairs * 4, pairs, size_t(M) * N * (out_type == 2 ? 4 : 2), 4};
+    const uintptr_t align[6] = {16, 16, 4, 1, uintptr_t(out_type == 2 ? 4 : 2), 4};
+    if (!buffers_ok(ptr, size, align, 4, 3)) return cudaErrorInvalidValue;  // zero points may be null
+    NvtxRange range("ornith.w4");
+    Args a{};
+    a.x = x, a.x_stride = x_stride;
+    a.tiles = static_cast<const uint4*>(tiles);
+    a.scales = static_cast<const uint32_t*>(tile_scales);
+    a.zeros = static_cast<const uint8_t*>(tile_zeros);
+    a.out = out, a.flags = static_cast<uint32_t*>(flags);
+    a.M = M, a.N = N, a.K = K, a.chunks = k_chunks(K), a.groups = groups;
+    a.group_shift = group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 8;
+    a.out_f32 = out_type == 2, a.scale_f16 = scale_type;
+    // Warps that share a row tile: as few as keep 16 warps on each SM.
+    a.split = 1;
+    while (a.split < kWarps && a.split < a.chunks && row_tiles(N) * a.split < kSms * 16) a.split *= 2;
+    const int per_cta = kWarps / a.split, blocks = (row_tiles(N) + per_cta - 1) / per_cta;
+    const bool zp = tile_zeros != nullptr, fine = group == 32;
+    count_launches(1);
+    if (x_type)
+        M <= 8 ? launch<true, 1>(a, zp, fine, blocks, stream) : launch<true, 2>(a, zp, fine, blocks, stream);
+    else
+        M <= 8 ? launch<false, 1>(a, zp, fine, blocks, stream) : launch<false, 2>(a, zp, fine, blocks, stream);
+    return cudaGetLastError();
+}

@@ -210,6 +210,60 @@ class W8HeadMethod(G256LinearMethod):
         return out.view(*x.shape[:-1], self.n)
 
 
+class W4LinearMethod(G256LinearMethod):
+    """A linear layer in the ordinary 4-bit checkpoint form: w4_codes uint32
+    [N, K/8], w4_scales [N, K/group] in params_dtype and, with zero_points,
+    w4_zeros uint8 [N, K/group].  Loading takes these; sealing lays them out
+    for the kernel and drops the checkpoint form; apply runs the rows 16 at a
+    time, in params_dtype (bf16 or fp16), with logits_fp32 into fp32 (a
+    vocabulary head for sampling)."""
+    fields = ('w4_codes', 'w4_scales', 'w4_zeros')
+
+    def __init__(self, prefix='', group=128, zero_points=False, logits_fp32=False):
+        super().__init__(prefix)
+        self.group, self.logits_fp32 = group, logits_fp32
+        if not zero_points:
+            self.fields = self.fields[:2]
+
+    def create_weights(self, layer, input_size_per_partition, output_partition_sizes, input_size, output_size,
+                       params_dtype, **attrs):
+        self.k, self.n, self.dtype = input_size, output_size, params_dtype
+        problems = [why for bad, why in (
+            (input_size_per_partition != input_size, 'a split input'),
+            (sum(output_partition_sizes) != output_size, 'output partitions that do not sum to the output'),
+            (getattr(layer, 'tp_size', 1) != 1, 'tensor parallelism'),
+            (params_dtype not in (torch.bfloat16, torch.float16), f'dtype {params_dtype}'),
+            (getattr(layer, 'has_bias', False), 'a bias'),
+        ) if bad]
+        if problems:
+            raise ValueError(f'4-bit linear {self.prefix}: unsupported geometry: {"; ".join(problems)}')
+        native.w4_pack_shapes(self.n, self.k, self.group)   # refuses other groups and sizes
+        groups = self.k // self.group
+        shapes = ((self.n, self.k // 8), (self.n, groups), (self.n, groups))
+        register_packed(layer, list(zip(self.fields, shapes, (torch.uint32, params_dtype, torch.uint8))),
+                        attrs.get('device'))
+
+    def process_weights_after_loading(self, layer):
+        super().process_weights_after_loading(layer)
+        layer._g256_ready = False
+        checkpoint = [getattr(layer, name).data for name in self.fields]
+        layer.w4_bank = native.w4_pack(*checkpoint)
+        for name in self.fields:
+            delattr(layer, name)
+        layer._g256_ready = True
+
+    def apply(self, layer, x, bias=None):
+        self._check_ready(layer, bias)
+        rows = x.reshape(-1, self.k).contiguous()
+        out = torch.empty((rows.shape[0], self.n), dtype=torch.float32 if self.logits_fp32 else rows.dtype,
+                          device=rows.device)
+        step = native.W4_ROWS
+        for first in range(0, rows.shape[0], step):
+            native.w4_out(rows[first:first + step], *layer.w4_bank, out[first:first + step],
+                          self.runtime.slots[self.slot], self.n, self.k)
+        return out.view(*x.shape[:-1], self.n)
+
+
 class G256MoEMethod:
     """The routed method of one MoE layer on this library.  `runtime` is an
     ornith_b200 Runtime (workspace arena, capacity, per-layer flag slots)

@@ -15,7 +15,13 @@ Mirrors the reference plugin's binding (plugin-site/ornith_g256/native.py):
     split of `ornith_g256::dense_out` (native.py:121-153), and
     `dense_n32_out` is the one-row N32 shadow launch of dense_n32.py:45-53;
   * `ornith_b200::head_out` is the W8 LM head launch of
-    `ornith_g256::head_out` (native.py:205-212).
+    `ornith_g256::head_out` (native.py:205-212);
+  * `ornith_b200::w4_out` is the product of 1 to 16 rows with a 4-bit weight
+    in the ordinary checkpoint form (group scales, zero points), laid out
+    once by `w4_pack`; the reference has no counterpart;
+  * `ornith_b200::sample_out` draws one token for each row of logits
+    (temperature, min-p, top-k, top-p) by a given random number; the reference
+    leaves this to vLLM.
 All launches go to the caller's current CUDA stream.  There is no CPU
 fallback: every operator raises if the CUDA library is missing.
 """
@@ -127,6 +133,11 @@ SIGNATURES = {
     'ornith_head_i8_tile_launch': ([C.c_void_p] * 4 + [C.c_size_t] + [C.c_void_p] * 2 + [C.c_size_t]
                                    + [C.c_void_p] + [C.c_int] * 4 + [C.c_void_p], C.c_int),
     'ornith_head_i8_tile_shortlist': ([], C.c_int),
+    'ornith_moe_b200_w4_pack': ([C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_void_p], C.c_int),
+    'ornith_moe_b200_w4_launch': ([C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                   C.c_void_p, C.c_int, C.c_void_p] + [C.c_int] * 4 + [C.c_void_p], C.c_int),
+    'ornith_moe_b200_sample_launch': ([C.c_void_p, C.c_int64, C.c_int] + [C.c_void_p] * 8 + [C.c_int] * 2
+                                      + [C.c_void_p], C.c_int),
 }
 
 
@@ -719,6 +730,179 @@ def head_launch(x, codes, scales, workspace, out, flags, n, capacity=HEAD_ROWS, 
     check(lib().ornith_head_i8_tile_launch(ptr(x), ptr(codes), ptr(scales), ptr(workspace), workspace.numel(),
                                            ptr(out), ptr(group_dots) if group_dots is not None else None, nbytes,
                                            ptr(flags), x.shape[0], capacity, n, geometry, stream(x)), 'W8 head')
+
+
+# ---------------------------------------------------------------------------
+# Matrix-vector products with 4-bit weights and group scales
+# ---------------------------------------------------------------------------
+W4_ROWS, W4_GROUPS, W4_MAX_K, W4_MAX_N = 16, (32, 64, 128, 256), 16384, 1 << 22
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def w4_pack_shapes(n, k, group):
+    """Shapes of the packed (tiles, scales, zero points) of an [n, k] weight."""
+    if group not in W4_GROUPS or not 0 < k <= W4_MAX_K or k % group or not 0 < n <= W4_MAX_N:
+        raise ValueError(f'a 4-bit weight has groups of 32, 64, 128 or 256, K a multiple of the group up to '
+                         f'{W4_MAX_K} and N up to {W4_MAX_N}; got N {n}, K {k}, group {group}')
+    row_tiles = -(-n // 16)
+    return (row_tiles, -(-k // 64), 32, 4), (row_tiles, k // group, 16), (row_tiles, k // group, 8)
+
+
+def w4_pack(codes, scales, zeros=None):
+    """Lay a 4-bit weight out for w4_launch, once when it is loaded.
+
+    codes uint32 [N, K/8] (value 8j + d of a row in bits 4d of its word j),
+    scales bf16 or fp16 [N, K/group], zeros uint8 [N, K/group] in 0..15 or None
+    for 8 everywhere.  Returns (tiles, scales, zeros) on the same device.
+    Reads the scales and zero points back to check them, so it is not for
+    stream capture."""
+    if (codes.dtype != torch.uint32 or codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0]
+            or scales.dtype not in (torch.bfloat16, torch.float16) or codes.device.type != 'cuda'
+            or scales.device != codes.device or not codes.is_contiguous() or not scales.is_contiguous()):
+        raise ValueError('w4_pack takes contiguous CUDA uint32 codes [N, K/8] and bf16 or fp16 scales [N, K/group]')
+    n, k, groups = codes.shape[0], codes.shape[1] * 8, scales.shape[1]
+    if not n or not groups or k % groups:
+        raise ValueError(f'w4_pack: {groups} scales a row do not divide K = {k}')
+    tile_shape, scale_shape, zero_shape = w4_pack_shapes(n, k, k // groups)
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape
+                              or zeros.device != codes.device or not zeros.is_contiguous()):
+        raise ValueError('w4_pack takes contiguous uint8 zero points of the shape of the scales')
+    if not bool(torch.isfinite(scales).all()) or (zeros is not None and int(zeros.max()) > 15):
+        raise ValueError('w4_pack: scales must be finite and zero points at most 15')
+    with torch.cuda.device(codes.device):
+        tiles = torch.empty(tile_shape, dtype=torch.uint32, device=codes.device)
+        tile_scales = torch.empty(scale_shape, dtype=scales.dtype, device=codes.device)
+        tile_zeros = None if zeros is None else torch.empty(zero_shape, dtype=torch.uint8, device=codes.device)
+        check(lib().ornith_moe_b200_w4_pack(ptr(codes), ptr(scales), ptr(zeros), ptr(tiles), ptr(tile_scales),
+                                            ptr(tile_zeros), n, k, k // groups, stream(codes)), 'W4 pack')
+    return tiles, tile_scales, tile_zeros
+
+
+def _launch_on(device, fn, *args):
+    """fn(*args, current stream of `device`) with that device current: the
+    caller's current device may be another one."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    with torch.cuda.device(index):
+        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+
+
+def w4_launch(x, tiles, scales, zeros, out, flags, n, k):
+    """out [M, n] (x's type or fp32) = x [M <= 16, k] (bf16 or fp16) times the
+    transposed weight [n, k] that w4_pack laid out as (tiles, scales, zeros).
+    x may have rows further apart than k (a multiple of 8 values, rows on 16
+    bytes).  flags receives the dense bits 4 (non-finite result) and 8
+    (non-finite stored value)."""
+    device = x.device
+    if (x.dim() != 2 or x.shape[1] != k or x.shape[0] > W4_ROWS or x.dtype not in (torch.bfloat16, torch.float16)
+            or device.type != 'cuda' or x.stride(1) != 1):
+        raise ValueError(f'w4_launch takes CUDA bf16 or fp16 rows [M <= {W4_ROWS}, {k}]')
+    m, stride = x.shape[0], x.stride(0)
+    if m and (x.data_ptr() % 16 or (m > 1 and (stride < k or stride % 8))):
+        raise ValueError('w4_launch takes rows that start on 16 bytes and do not overlap')
+    if (out.shape != (m, n) or (out.dtype != x.dtype and out.dtype != torch.float32) or out.device != device
+            or not out.is_contiguous()):
+        raise ValueError(f'w4_launch writes a contiguous [M, {n}] of the type of x or fp32 on the device of x')
+    groups = scales.shape[1] if scales.dim() == 3 else 0
+    if not groups or k % groups:
+        raise ValueError('w4_launch takes the scales that w4_pack returned')
+    tile_shape, scale_shape, zero_shape = w4_pack_shapes(n, k, k // groups)
+    if (tiles.shape != tile_shape or tiles.dtype != torch.uint32 or scales.shape != scale_shape
+            or scales.dtype not in (torch.bfloat16, torch.float16) or tiles.device != device
+            or scales.device != device or not tiles.is_contiguous() or not scales.is_contiguous()
+            or (zeros is not None and (zeros.shape != zero_shape or zeros.dtype != torch.uint8
+                                       or zeros.device != device or not zeros.is_contiguous()))):
+        raise ValueError(f'w4_launch takes tiles, scales and zero points as w4_pack returns them for [{n}, {k}]')
+    _check_flags(flags, device)
+    check(_launch_on(device, lib().ornith_moe_b200_w4_launch, x.data_ptr(), stride, _TYPES[x.dtype],
+                     tiles.data_ptr(), scales.data_ptr(), _TYPES[scales.dtype],
+                     None if zeros is None else zeros.data_ptr(), out.data_ptr(), _TYPES[out.dtype],
+                     flags.data_ptr(), m, n, k, k // groups), 'W4 product')
+
+
+def _check_flags(flags, device):
+    if flags.dtype != torch.int32 or flags.numel() != 1 or flags.device != device:
+        raise ValueError('flags is one int32 word on the device of the input')
+
+
+@torch.library.custom_op('ornith_b200::w4_out', mutates_args={'out', 'flags'}, device_types='cuda')
+def w4_out(x: torch.Tensor, tiles: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None,
+           out: torch.Tensor, flags: torch.Tensor, n: int, k: int) -> None:
+    """w4_launch as a torch operator."""
+    w4_launch(x, tiles, scales, zeros, out, flags, n, k)
+
+
+@w4_out.register_fake
+def _w4_fake(x, tiles, scales, zeros, out, flags, n, k):
+    return None
+
+
+# ---------------------------------------------------------------------------
+# Token sampling
+# ---------------------------------------------------------------------------
+SAMPLE_MAX_VOCAB = 1 << 19
+
+
+def sample_launch(logits, temperature, top_k, top_p, min_p, uniform, tokens, logprobs, flags):
+    """One token for each row of logits [M, V <= 524288] (bf16, fp16 or fp32;
+    rows may be further apart than V).
+
+    With w_i = exp((x_i - max x) / temperature): min-p keeps w_i >= min_p, then
+    top-k the first k by (logit, lowest index first), then top-p the smallest
+    prefix of those, in that order, with top_p of their mass (one token at
+    least); tokens int32 [M] gets the first kept index whose running sum, in
+    index order, exceeds uniform times the kept mass.  temperature 0 takes the
+    largest logit, lowest index.
+
+    temperature, top_p, min_p, uniform: fp32 [M]; top_k: int32 [M]; all but
+    uniform may be None (temperature 1, no cut); top_k < 1 or >= V, top_p >= 1
+    and min_p 0 switch their cut off for a row.  logprobs fp32 [M] or None: the
+    model's own log probability of the token, over all tokens at temperature 1.
+
+    A row that cannot be sampled gets token -1 and log probability NaN and
+    raises a bit of flags: 1 NaN or +inf among its logits, 2 a parameter out of
+    range (temperature outside [0, 1e30], negative top_p, min_p outside [0, 1],
+    uniform outside [0, 1), any NaN), 4 every logit -inf."""
+    device = logits.device
+    if (logits.dim() != 2 or logits.dtype not in _TYPES or device.type != 'cuda'
+            or not 0 < logits.shape[1] <= SAMPLE_MAX_VOCAB
+            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+        raise ValueError(f'sample_launch takes CUDA bf16, fp16 or fp32 logits [M, V <= {SAMPLE_MAX_VOCAB}] with '
+                         'neighbouring values')
+    m, vocab = logits.shape
+    stride = logits.stride(0) if m > 1 else vocab
+    if stride < vocab:
+        raise ValueError('sample_launch takes rows that do not overlap')
+    for name, t, dtype, optional in (('temperature', temperature, torch.float32, True),
+                                     ('top_k', top_k, torch.int32, True), ('top_p', top_p, torch.float32, True),
+                                     ('min_p', min_p, torch.float32, True),
+                                     ('uniform', uniform, torch.float32, False),
+                                     ('tokens', tokens, torch.int32, False),
+                                     ('logprobs', logprobs, torch.float32, True)):
+        if t is None and optional:
+            continue
+        if t is None or t.dtype != dtype or t.shape != (m,) or t.device != device or not t.is_contiguous():
+            raise ValueError(f'sample_launch takes {name} as a contiguous {dtype} [{m}] on the device of the logits')
+    _check_flags(flags, device)
+    check(_launch_on(device, lib().ornith_moe_b200_sample_launch, logits.data_ptr(), stride, _TYPES[logits.dtype],
+                     *[None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p, uniform,
+                                                                     tokens, logprobs, flags)],
+                     m, vocab), 'sampling')
+
+
+@torch.library.custom_op('ornith_b200::sample_out', mutates_args={'tokens', 'logprobs', 'flags'},
+                         device_types='cuda')
+def sample_out(logits: torch.Tensor, temperature: torch.Tensor | None, top_k: torch.Tensor | None,
+               top_p: torch.Tensor | None, min_p: torch.Tensor | None, uniform: torch.Tensor, tokens: torch.Tensor,
+               logprobs: torch.Tensor | None, flags: torch.Tensor) -> None:
+    """sample_launch as a torch operator."""
+    sample_launch(logits, temperature, top_k, top_p, min_p, uniform, tokens, logprobs, flags)
+
+
+@sample_out.register_fake
+def _sample_fake(logits, temperature, top_k, top_p, min_p, uniform, tokens, logprobs, flags):
+    return None
 
 
 # ---------------------------------------------------------------------------

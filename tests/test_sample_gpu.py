@@ -1,0 +1,305 @@
+"""GPU: token sampling against its definition in 64 bits.
+
+Tokens are compared exactly: the weights' relative error (below 1e-13) moves a
+border between two tokens past a given random number with a probability below
+1e-9 a row.  A log probability is off by the sum of at most 68 fp32 terms in a
+thread, each exact to two steps (72 steps of 2^-24 relative in all, the same
+absolutely after the logarithm), and by half a step of its own."""
+import importlib
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device('cuda:0')
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def sample_row(x, T, k, p, min_p, u):
+    """The definition for one row in 64 bits."""
+    x = x.astype(np.float64)
+    if not (0 <= T <= float(np.float32(1e30))) or not p >= 0 or not 0 <= min_p <= 1 or not 0 <= u < 1:
+        return -1, math.nan, 2
+    if np.isnan(x).any() or x.max() == np.inf:
+        return -1, math.nan, 1
+    top = x.max()
+    if top == -np.inf:
+        return -1, math.nan, 4
+    if T == 0:
+        token = int(np.argmax(x))
+    else:
+        with np.errstate(over='ignore', under='ignore'):
+            w = np.exp((x - top) / T)
+        order = np.argsort(-x, kind='stable')
+        order = order[(w[order] >= min_p) & (x[order] > -np.inf)]
+        if 0 < k < len(order):
+            order = order[:k]
+        if p < 1:
+            cum = np.cumsum(w[order])
+            order = order[:1 + int(np.searchsorted(cum[:-1], p * cum[-1]))]
+        kept = np.sort(order)
+        cum = np.cumsum(w[kept])
+        token = int(kept[np.searchsorted(cum, u * cum[-1], side='right')])
+    with np.errstate(under='ignore'):
+        logp = x[token] - top - math.log(np.exp(x - top).sum())
+    return token, logp, 0
+
+
+def run(native, logits, T=None, k=None, p=None, min_p=None, u=None, want_logp=True):
+    m = logits.shape[0]
+    f = lambda v, dtype: None if v is None else torch.as_tensor(v, dtype=dtype).expand(m).contiguous().to(DEV)  # noqa: E731
+    tokens = torch.full((m,), -7, dtype=torch.int32, device=DEV)
+    logp = torch.full((m,), 7.0, device=DEV) if want_logp else None
+    flags = torch.zeros(1, dtype=torch.int32, device=DEV)
+    native.sample_launch(logits, f(T, FP32), f(k, torch.int32), f(p, FP32), f(min_p, FP32),
+                         f(0.5 if u is None else u, FP32), tokens, logp, flags)
+    return tokens, logp, flags
+
+
+def check(native, logits, T=None, k=None, p=None, min_p=None, u=None):
+    m = logits.shape[0]
+    tokens, logp, flags = run(native, logits, T, k, p, min_p, u)
+    x = logits.double().cpu().numpy()
+    par = [np.broadcast_to(np.asarray(torch.as_tensor(d if v is None else v, dtype=FP32).double()), (m,))
+           for v, d in ((T, 1.0), (p, 1.0), (min_p, 0.0), (u, 0.5))]
+    ks = np.broadcast_to(np.asarray(0 if k is None else k), (m,))
+    tokens, logp, want_flags = tokens.cpu().numpy(), logp.cpu().numpy(), 0
+    for r in range(m):
+        token, lp, flag = sample_row(x[r], par[0][r], int(ks[r]), par[1][r], par[2][r], par[3][r])
+        want_flags |= flag
+        assert tokens[r] == token, (r, tokens[r], token)
+        if math.isnan(lp):
+            assert math.isnan(logp[r])
+        else:
+            assert abs(logp[r] - lp) <= 72 * 2.0 ** -24 + 2.0 ** -24 * abs(lp), (r, logp[r], lp)
+    assert int(flags) == want_flags
+
+
+def logits_of(m, vocab, dtype, seed, spread=2.0, head=0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((m, vocab), generator=gen) * spread
+    if head:
+        at = torch.randint(0, vocab, (m, head), generator=gen)
+        x.scatter_(1, at, 16.0 - 2.0 * torch.arange(1, head + 1).float().log().expand(m, head))
+    return x.to(dtype).to(DEV)
+
+
+def uniform(m, seed):
+    return torch.rand(m, generator=torch.Generator().manual_seed(seed))
+
+
+SETTINGS = [dict(), dict(T=0.7), dict(k=5), dict(k=300), dict(p=0.9), dict(p=0.2), dict(min_p=0.1), dict(T=0.0),
+            dict(T=1.5, k=50, p=0.8), dict(T=0.6, k=1000, p=0.95, min_p=0.01), dict(T=30.0, p=0.5),
+            dict(T=30.0, k=777), dict(T=0.01, p=0.9), dict(k=1), dict(p=0.0), dict(min_p=1.0), dict(p=0.99999)]
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('vocab', [1, 2, 7, 33, 1003, 4099])
+def test_small_vocabularies(native, vocab, dtype):
+    for i, s in enumerate(SETTINGS):
+        check(native, logits_of(9, vocab, dtype, i), u=uniform(9, 100 + i), **s)
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('head', [0, 100])
+def test_settings(native, dtype, head):
+    for i, s in enumerate(SETTINGS):
+        check(native, logits_of(3, 50257, dtype, i, head=head), u=uniform(3, i), **s)
+
+
+@pytest.mark.parametrize('m,vocab,dtype', [(1, 248320, BF16), (2, 248320, FP32), (20, 248320, BF16),
+                                           (1, 524288, FP32), (2, 524287, FP16), (70, 65536, FP32), (500, 256, BF16)])
+def test_sizes(native, m, vocab, dtype):
+    """One to sixteen CTAs a row, with rows enough to fill the GPU and without."""
+    x = logits_of(m, vocab, dtype, 3, head=64)
+    for i, s in enumerate((dict(), dict(T=0.8, k=40, p=0.95), dict(T=2.0, p=0.9), dict(T=1.2, k=20000, min_p=1e-6))):
+        check(native, x, u=uniform(m, i), **s)
+
+
+def test_row_parameters(native):
+    m = 48
+    gen = torch.Generator().manual_seed(5)
+    r = lambda: torch.rand(m, generator=gen)  # noqa: E731
+    T = torch.where(r() < 0.2, 0.0, 2 * r())
+    k = torch.where(r() < 0.3, 0.0, torch.exp(r() * 8)).int()
+    k[0], k[1] = -5, 2 ** 31 - 1
+    p = torch.where(r() < 0.3, 1.5, r())
+    min_p = torch.where(r() < 0.5, 0.0, 0.5 * r())
+    check(native, logits_of(m, 32003, BF16, 1, head=30), T, k, p, min_p, r())
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+def test_ties(native, dtype):
+    """Rows of few distinct logits: a border inside thousands of equal values goes by index."""
+    x = logits_of(6, 70001, FP32, 8).round().to(dtype)
+    x[1] = 0.25                                                     # one value
+    x[2] = torch.where(x[2] > 3, 1.0, 0.0).to(dtype)                # two
+    for i, s in enumerate((dict(k=1), dict(k=35000), dict(k=70000), dict(p=0.5), dict(p=0.25, k=60001),
+                           dict(T=0.5, p=0.9), dict(min_p=0.3, p=0.7), dict(T=3.0, k=2000, p=0.5), dict())):
+        check(native, x, u=uniform(6, i), **s)
+    # an even row cut in half: the border falls exactly between two tokens
+    even = torch.zeros((1, 1000), dtype=dtype, device=DEV)
+    for u in (0.0, 0.5, 1 - 2.0 ** -24):
+        assert int(run(native, even, p=0.5, u=u)[0]) == int(500 * u)
+
+
+def test_random_numbers_at_the_ends(native):
+    last = 1 - 2.0 ** -24
+    for dtype in (BF16, FP32):
+        x = logits_of(4, 9973, dtype, 2, spread=20.0)
+        for u in (0.0, 2.0 ** -30, last):
+            for s in (dict(), dict(p=0.9), dict(k=3), dict(T=5.0, p=0.999)):
+                check(native, x, u=u, **s)
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+def test_masks(native, dtype):
+    lowest = torch.finfo(dtype).min
+    base = logits_of(8, 20011, dtype, 4)
+    gone = torch.rand(base.shape, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for mask in (-math.inf, lowest):
+        x = base.clone()
+        for r, share in enumerate((0.0, 0.5, 0.99, 0.9999)):
+            x[r] = torch.where(gone[r] < share, mask, x[r].float()).to(dtype)
+        x[4, 1:] = mask                       # the first token alone
+        x[5, :-1] = mask                      # the last
+        x[6] = mask                           # nothing left, or all alike
+        x[7, 100:] = -math.inf
+        x[7, :50] = lowest                    # both masks
+        for i, s in enumerate((dict(), dict(k=50), dict(p=0.9), dict(T=0.0), dict(min_p=0.2), dict(T=1e5, k=10),
+                               dict(T=1e5, p=0.5), dict(T=1e30), dict(T=1e-30, p=0.5), dict(T=1e30, k=15000, p=0.3))):
+            check(native, x, u=uniform(8, i), **s)
+
+
+def test_bad_rows_are_refused_alone(native):
+    x = logits_of(12, 5000, FP32, 6)
+    x[1, 4999], x[3, 0], x[5] = math.nan, math.inf, -math.inf
+    T, p, min_p, u = torch.ones(12), torch.full((12,), 0.9), torch.zeros(12), uniform(12, 3)
+    check(native, x[[0, 1]], T[:2], p=p[:2], u=u[:2])
+    check(native, x[[0, 3]], T[:2], p=p[:2], u=u[:2])
+    check(native, x[[0, 5]], T[:2], p=p[:2], u=u[:2])
+    for name, value in (('T', -1.0), ('T', math.nan), ('T', math.inf), ('p', -0.1), ('p', math.nan),
+                        ('min_p', 1.5), ('min_p', math.nan), ('min_p', -0.1), ('u', 1.0), ('u', -0.5),
+                        ('u', math.nan)):
+        par = dict(T=T.clone(), p=p.clone(), min_p=min_p.clone(), u=u.clone())
+        par[name][7] = value
+        check(native, x, **par)
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+def test_strides_and_alignment(native, dtype):
+    """Rows that start anywhere inside a 16-byte vector, out of a wider tensor whose other values are NaN."""
+    wide = torch.full((5, 3050), math.nan, dtype=dtype, device=DEV)
+    values = logits_of(5, 3001, dtype, 9)
+    for offset in range(0, 9):
+        wide.fill_(math.nan)
+        view = wide[:, offset:offset + 3001]
+        view.copy_(values)
+        for s in (dict(), dict(k=20, p=0.9), dict(T=0.0)):
+            check(native, view, u=uniform(5, offset), **s)
+    check(native, wide[2:3, 8:3009], u=[0.3])
+
+
+def test_same_token_whatever_the_launch_shape(native):
+    """A row alone (many CTAs) and among many (few CTAs)."""
+    row = logits_of(1, 131072, FP32, 11)
+    many = row.expand(200, -1).contiguous()
+    for i, s in enumerate((dict(), dict(T=1.3, p=0.93), dict(T=2.0, k=9000, p=0.8))):
+        u = float(uniform(1, 20 + i))
+        one, logp, _ = run(native, row, u=u, **s)
+        tokens, _, _ = run(native, many, u=u, **s)
+        assert bool((tokens == one).all())
+
+
+def test_frequencies(native):
+    """Tokens come with their probabilities: a stratified set of random numbers hits each token's share exactly."""
+    x = logits_of(1, 50, FP32, 12, spread=1.0)
+    n = 4096
+    u = (torch.arange(n) + 0.5) / n
+    tokens, _, _ = run(native, x.expand(n, -1).contiguous(), p=0.8, u=u)
+    w = torch.softmax(x.double(), 1)[0].cpu()
+    order = w.argsort(descending=True)
+    kept = order[:1 + int((w[order].cumsum(0)[:-1] < 0.8).sum())]
+    share = torch.zeros(50, dtype=torch.float64)
+    share[kept] = w[kept] / w[kept].sum()
+    count = torch.bincount(tokens.cpu().long(), minlength=50)
+    assert bool(((count - n * share).abs() <= 1).all())   # an interval holds its length in grid points, give or take one
+
+
+def test_without_logprobs_on_a_stream_and_captured(native):
+    x = logits_of(4, 30000, BF16, 13)
+    u = uniform(4, 1).to(DEV)
+    tokens = torch.zeros(4, dtype=torch.int32, device=DEV)
+    logp = torch.zeros(4, device=DEV)
+    flags = torch.zeros(1, dtype=torch.int32, device=DEV)
+    p = torch.full((4,), 0.9, device=DEV)
+    want, want_logp, _ = run(native, x, p=p, u=u)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        native.sample_launch(x, None, None, p, None, u, tokens, None, flags)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(tokens, want)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for graph in graphs:                                    # two graphs over the same buffers
+        with torch.cuda.graph(graph):
+            native.sample_out(x, None, None, p, None, u, tokens, logp, flags)
+    x.copy_(logits_of(4, 30000, BF16, 14))
+    want, want_logp, _ = run(native, x, p=p, u=u)
+    for graph in graphs:
+        tokens.zero_()
+        graph.replay()
+        assert torch.equal(tokens, want) and torch.equal(logp, want_logp)
+
+
+def test_no_rows_and_refusals(native):
+    x = logits_of(3, 100, FP32, 1)
+    u = uniform(3, 1).to(DEV)
+    tokens = torch.zeros(3, dtype=torch.int32, device=DEV)
+    logp = torch.zeros(3, device=DEV)
+    flags = torch.zeros(1, dtype=torch.int32, device=DEV)
+    native.sample_launch(x[:0], None, None, None, None, u[:0], tokens[:0], logp[:0], flags)
+    good = dict(logits=x, temperature=u, top_k=tokens.clone(), top_p=u, min_p=u, uniform=u, tokens=tokens,
+                logprobs=logp, flags=flags)
+    native.sample_launch(**good)
+    bad = [dict(logits=x.double()), dict(logits=x[0]), dict(logits=x.t()), dict(logits=x[:1].expand(3, 100)),
+           dict(logits=x.cpu()), dict(logits=x[:, :0]), dict(logits=torch.zeros((3, (1 << 19) + 1), device=DEV)),
+           dict(temperature=u.double()), dict(top_k=tokens.long()), dict(top_p=u[:2]), dict(min_p=u.cpu()),
+           dict(uniform=None), dict(uniform=u[:, None]), dict(tokens=tokens.long()), dict(tokens=None),
+           dict(logprobs=logp.double()), dict(flags=flags.long()),
+           dict(tokens=torch.zeros(6, dtype=torch.int32, device=DEV)[::2])]
+    for change in bad:
+        with pytest.raises(ValueError):
+            native.sample_launch(**{**good, **change})
+    with pytest.raises(RuntimeError):
+        native.sample_launch(**{**good, 'logprobs': u})     # written over an input
+
+
+def test_hidden_states_to_tokens(native):
+    """The end of a decode step as a server runs it: a 4-bit head in its layer method, then the sampler."""
+    method = importlib.import_module('ornith_b200.method')
+    runtime = importlib.import_module('ornith_b200.runtime')
+    n, k, m = 32000, 2048, 20
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    codes = torch.randint(-2 ** 31, 2 ** 31, (n, k // 8), dtype=torch.int32, device=DEV, generator=gen)
+    scales = (0.01 * torch.rand((n, k // 128), device=DEV, generator=gen)).to(BF16)
+    layer = torch.nn.Module()
+    head = method.W4LinearMethod('head', group=128, logits_fp32=True)
+    head.create_weights(layer, k, [n], k, n, BF16, device=DEV)
+    layer.w4_codes.weight_loader(layer.w4_codes, codes.view(torch.uint32))
+    layer.w4_scales.weight_loader(layer.w4_scales, scales)
+    head.process_weights_after_loading(layer)
+    rt = runtime.Runtime(['head', 'sampler'], 32, DEV)
+    head.bind(rt, 0)
+    x = torch.randn((m, k), device=DEV, generator=gen).to(BF16)
+    logits = head.apply(layer, x)
+    shift = torch.arange(0, 32, 4, dtype=torch.int32, device=DEV)
+    weight = (((codes[:, :, None] >> shift) & 15).view(n, k // 128, 128).double() - 8) * scales.double()[:, :, None]
+    want = x.double() @ weight.view(n, k).t()
+    assert float((logits.double() - want).norm() / want.norm()) < 1e-6   # 200 steps of 2^-24, as a random walk
+    check(native, logits, T=0.8, k=50, p=0.95, u=uniform(m, 7))
+    tokens = torch.empty(m, dtype=torch.int32, device=DEV)
+    native.sample_out(logits, None, None, None, None, uniform(m, 8).to(DEV), tokens, None, rt.slots[1])
+    assert bool(((tokens >= 0) & (tokens < n)).all()) and rt.check_error_flags() == [0, 0]
