@@ -114,41 +114,41 @@ struct Args {
     const uint8_t* zeros;
     void* out;
     uint32_t* flags;
-    int M, N, K, chunks, groups, group_shift, split, out_f32, scale_f16;
+    // per_warp: chunks of one warp, a multiple of a group's; split: warps that share a row tile
+    int M, N, K, chunks, groups, per_warp, split, out_f32, scale_f16;
 };
 
+// A fragment register as the codes' exponent trick leaves it, 128 + c (bf16) or
+// 1024 + c (fp16) in each half, and the exact step down to c - z: one FMA with
+// one and -(128 + z) or -(1024 + z).
 template <bool F16>
-struct Num;
-template <>
-struct Num<false> {  // bf16: 128 + c has c in the low mantissa bits
-    static constexpr uint32_t kMagic = 0x43004300u;
-    static __device__ __forceinline__ uint32_t bias(uint32_t z) { return kMagic | z | z << 16; }
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+struct Num {
+    static constexpr uint32_t kMagic = F16 ? 0x64006400u : 0x43004300u;
+    static constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
+    static __device__ __forceinline__ uint32_t bias(uint32_t z) { return (z * 0x10001u) | kMagic | 0x80008000u; }
+    static __device__ __forceinline__ uint32_t centred(uint32_t v, uint32_t bias) {
         uint32_t d;
-        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        if (F16)
+            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(v), "r"(kOne), "r"(bias));
+        else
+            asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(v), "r"(kOne), "r"(bias));
         return d;
     }
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-template <>
-struct Num<true> {  // fp16: 1024 + c
-    static constexpr uint32_t kMagic = 0x64006400u;
-    static __device__ __forceinline__ uint32_t bias(uint32_t z) { return kMagic | z | z << 16; }
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        uint32_t d;
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-        return d;
-    }
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                               bool opens) {
+        const float c[4] = {opens ? 0.f : d[0], opens ? 0.f : d[1], opens ? 0.f : d[2], opens ? 0.f : d[3]};
+        if (F16)
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                "{%10,%11,%12,%13};"
+                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
+                  "f"(c[3]));
+        else
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                "{%10,%11,%12,%13};"
+                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
+                  "f"(c[3]));
     }
 };
 
@@ -166,90 +166,103 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
 }
 
 // kWarps warps; `split` warps (a power of two up to kWarps) share a row tile,
-// taking its chunks in turn, and join their sums through shared memory.
-// MT: tiles of 8 activation rows; FINE: groups of 32, two runs per chunk.
-template <bool F16, int MT, bool ZP, bool FINE>
+// each with a range of its chunks, and join their sums through shared memory.
+// MT: tiles of 8 activation rows.  Rows past M repeat the last one: columns of
+// the product are independent and theirs are not stored.
+template <bool F16, int MT, bool ZP, int GROUP>
 __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
-    constexpr int kAhead = 4, kRuns = FINE ? 2 : 1;
+    constexpr int kAhead = 4;                              // chunks in flight
+    constexpr int kRuns = GROUP == 32 ? 2 : 1;             // groups in a chunk
+    constexpr int kSpan = GROUP < 64 ? 1 : GROUP / 64;     // chunks of a group
+    constexpr int kMeta = kAhead / kSpan;                  // scales in flight, per run
     __shared__ float joined[kWarps][16][8 * MT + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
     const int part = warp & (a.split - 1);
     const int per_cta = kWarps / a.split;
     const int row_tile = blockIdx.x * per_cta + warp / a.split;
-    const int n_tiles = (a.N + 15) / 16;
+    const int first = part * a.per_warp;
+    int left = row_tile < (a.N + 15) / 16 ? min(a.per_warp, a.chunks - first) : 0;
     float acc[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
 
-    if (row_tile < n_tiles) {
-        const uint4* tile = a.tiles + size_t(row_tile) * a.chunks * 32 + lane;
-        const uint32_t* scale = a.scales + size_t(row_tile) * a.groups * 8 + r;
-        const uint8_t* zero = ZP ? a.zeros + size_t(row_tile) * a.groups * 8 + r : nullptr;
-        const uint16_t* xrow[MT];
-        bool has[MT];
+    if (left > 0) {
+        const uint4* tile = a.tiles + (size_t(row_tile) * a.chunks + first) * 32 + lane;
+        const size_t meta = (size_t(row_tile) * a.groups + first / kSpan * kRuns) * 8 + r;
+        const uint32_t* scale = a.scales + meta;
+        const uint8_t* zero = ZP ? a.zeros + meta : nullptr;
+        const uint16_t* x[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            has[i] = 8 * i + r < a.M;
-            xrow[i] = static_cast<const uint16_t*>(a.x) + (has[i] ? (8 * i + r) * a.x_stride : 0) + 8 * t;
-        }
+        for (int i = 0; i < MT; ++i)
+            x[i] = static_cast<const uint16_t*>(a.x) + min(8 * i + r, a.M - 1) * a.x_stride + 64 * first + 8 * t;
+        // a K of 32 more than a multiple of 64 ends in half a chunk, without the second group
+        int halves = GROUP == 32 ? a.K / 32 - 2 * first : 0;
         uint4 code[kAhead];
-        uint32_t sc[kAhead][kRuns], zp[kAhead][kRuns];
-        auto fetch = [&](int slot, int c) {
-            if (c >= a.chunks) return;
-            code[slot] = load_stream(tile + size_t(c) * 32);
+        uint32_t sc[kMeta][kRuns], zp[kMeta][kRuns];
+        // chunk d of the next kAhead, `at` chunks further on; the first chunk of a group brings its scale
+        auto fetch = [&](int d, int at) {
+            code[d] = load_stream(tile + (at + d) * 32);
+            if (d % kSpan == 0) {
 #pragma unroll
-            for (int h = 0; h < kRuns; ++h) {
-                // the last chunk of a K that is 32 more than a multiple of 64 has one group
-                const int g = min((64 * c + 32 * h) >> a.group_shift, a.groups - 1);
-                sc[slot][h] = __ldg(scale + g * 8);
-                zp[slot][h] = ZP ? uint32_t(__ldg(zero + g * 8)) : 0x88u;
+                for (int h = 0; h < kRuns; ++h)
+                    if (h == 0 || halves > 2 * (at + d) + h) {
+                        const int g = (at + d) / kSpan * kRuns + h;
+                        sc[d / kSpan][h] = __ldg(scale + g * 8);
+                        if (ZP) zp[d / kSpan][h] = __ldg(zero + g * 8);
+                    }
             }
         };
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d) fetch(d, part + d * a.split);
-        for (int base = part; base < a.chunks; base += kAhead * a.split) {
+        for (int d = 0; d < kAhead; ++d)
+            if (d < left) fetch(d, 0);
+        float run[MT][4];
+        while (left > 0) {
 #pragma unroll
             for (int d = 0; d < kAhead; ++d) {
-                const int c = base + d * a.split;
-                if (c >= a.chunks) break;
+                if (d >= left) break;
                 const uint32_t word[4] = {code[d].x, code[d].y, code[d].z, code[d].w};
-                uint32_t s2[kRuns], z2[kRuns];
+                uint32_t s2[kRuns];
+                uint32_t bias_lo[kRuns], bias_hi[kRuns];
 #pragma unroll
-                for (int h = 0; h < kRuns; ++h) s2[h] = sc[d][h], z2[h] = zp[d][h];
-                fetch(d, c + kAhead * a.split);
-                float run[MT][4];
+                for (int h = 0; h < kRuns; ++h) {
+                    s2[h] = sc[d / kSpan][h];
+                    const uint32_t z = ZP ? zp[d / kSpan][h] : 0x88u;
+                    bias_lo[h] = Num<F16>::bias(z & 15u), bias_hi[h] = Num<F16>::bias(z >> 4);
+                }
+                // the group's scale is still needed by its later chunks: fetch after its last
+                uint4 b[2][MT];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (FINE && 64 * c + 32 * h >= a.K) break;  // the same for the whole warp
-                    uint4 b[MT];
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
-                        b[i] = has[i] ? __ldg(reinterpret_cast<const uint4*>(xrow[i] + 64 * c + 32 * h))
-                                      : make_uint4(0u, 0u, 0u, 0u);
-                    const uint32_t z = z2[FINE ? h : 0];
-                    const uint32_t bias_lo = Num<F16>::bias(z & 15u), bias_hi = Num<F16>::bias(z >> 4);
-                    if (h == 0 || FINE) {
+                        if (h == 0 || GROUP != 32 || halves > 2 * d + h)
+                            b[h][i] = __ldg(reinterpret_cast<const uint4*>(x[i] + 64 * d + 32 * h));
+                if (d % kSpan == kSpan - 1) {
 #pragma unroll
-                        for (int i = 0; i < MT; ++i)
+                    for (int e = d - kSpan + 1; e <= d; ++e)
+                        if (left > kAhead + e) fetch(e, kAhead);
+                }
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) run[i][j] = 0.f;
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    if (GROUP == 32 && h == 1 && halves <= 2 * d + 1) break;  // the same for the whole warp
+                    const int g = kRuns == 2 ? h : 0;
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
                         uint32_t frag[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            frag[j] = Num<F16>::sub(((word[2 * h + p] >> (4 * j)) & 0x000f000fu) | Num<F16>::kMagic,
-                                                    j & 1 ? bias_hi : bias_lo);
+                            frag[j] = Num<F16>::centred(((word[2 * h + p] >> (4 * j)) & 0x000f000fu) | Num<F16>::kMagic,
+                                                        j & 1 ? bias_hi[g] : bias_lo[g]);
+                        const bool opens = p == 0 && (kRuns == 2 || (h == 0 && d % kSpan == 0));
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
-                            Num<F16>::mma(run[i], frag, p ? b[i].z : b[i].x, p ? b[i].w : b[i].y);
+                            Num<F16>::mma(run[i], frag, p ? b[h][i].z : b[h][i].x, p ? b[h][i].w : b[h][i].y, opens);
                     }
-                    if (h == 1 || FINE) {
-                        const uint32_t s = s2[FINE ? h : 0];
-                        const float lo = scale_value(s & 0xffffu, a.scale_f16), hi = scale_value(s >> 16, a.scale_f16);
+                    if (kRuns == 2 || (h == 1 && d % kSpan == kSpan - 1)) {
+                        const float lo = scale_value(s2[g] & 0xffffu, a.scale_f16);
+                        const float hi = scale_value(s2[g] >> 16, a.scale_f16);
 #pragma unroll
                         for (int i = 0; i < MT; ++i) {
                             acc[i][0] = __fmaf_rn(lo, run[i][0], acc[i][0]);
@@ -260,6 +273,11 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
                     }
                 }
             }
+            left -= kAhead, halves -= 2 * kAhead;
+            tile += kAhead * 32, scale += kMeta * kRuns * 8;
+            if (ZP) zero += kMeta * kRuns * 8;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[i] += kAhead * 64;
         }
     }
 #pragma unroll
@@ -291,10 +309,12 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
     if (fault) atomicOr(a.flags, fault);
 }
 
-template <bool F16, int MT>
-void launch(const Args& a, bool zp, bool fine, int blocks, cudaStream_t stream) {
-    auto* kernel = zp ? (fine ? w4_matvec_kernel<F16, MT, true, true> : w4_matvec_kernel<F16, MT, true, false>)
-                      : (fine ? w4_matvec_kernel<F16, MT, false, true> : w4_matvec_kernel<F16, MT, false, false>);
+template <bool F16, int MT, bool ZP>
+void launch(const Args& a, int group, int blocks, cudaStream_t stream) {
+    auto* kernel = group == 32    ? w4_matvec_kernel<F16, MT, ZP, 32>
+                   : group == 64  ? w4_matvec_kernel<F16, MT, ZP, 64>
+                   : group == 128 ? w4_matvec_kernel<F16, MT, ZP, 128>
+                                  : w4_matvec_kernel<F16, MT, ZP, 256>;
     kernel<<<blocks, kWarps * 32, 0, stream>>>(a);
 }
 
@@ -360,17 +380,19 @@ extern "C" cudaError_t ornith_moe_b200_w4_launch(const void* x, int64_t x_stride
     a.zeros = static_cast<const uint8_t*>(tile_zeros);
     a.out = out, a.flags = static_cast<uint32_t*>(flags);
     a.M = M, a.N = N, a.K = K, a.chunks = k_chunks(K), a.groups = groups;
-    a.group_shift = group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 8;
     a.out_f32 = out_type == 2, a.scale_f16 = scale_type;
     // Warps that share a row tile: as few as keep 16 warps on each SM.
+    const int span = group < 64 ? 1 : group / 64, units = (a.chunks + span - 1) / span;
     a.split = 1;
-    while (a.split < kWarps && a.split < a.chunks && row_tiles(N) * a.split < kSms * 16) a.split *= 2;
+    while (a.split < kWarps && a.split < units && row_tiles(N) * a.split < kSms * 16) a.split *= 2;
+    a.per_warp = (units + a.split - 1) / a.split * span;
     const int per_cta = kWarps / a.split, blocks = (row_tiles(N) + per_cta - 1) / per_cta;
-    const bool zp = tile_zeros != nullptr, fine = group == 32;
     count_launches(1);
-    if (x_type)
-        M <= 8 ? launch<true, 1>(a, zp, fine, blocks, stream) : launch<true, 2>(a, zp, fine, blocks, stream);
-    else
-        M <= 8 ? launch<false, 1>(a, zp, fine, blocks, stream) : launch<false, 2>(a, zp, fine, blocks, stream);
+    using Launch = void (*)(const Args&, int, int, cudaStream_t);
+    static constexpr Launch table[2][2][2] = {{{launch<false, 1, false>, launch<false, 1, true>},
+                                               {launch<false, 2, false>, launch<false, 2, true>}},
+                                              {{launch<true, 1, false>, launch<true, 1, true>},
+                                               {launch<true, 2, false>, launch<true, 2, true>}}};
+    table[x_type][M > 8][tile_zeros != nullptr](a, group, blocks, stream);
     return cudaGetLastError();
 }
