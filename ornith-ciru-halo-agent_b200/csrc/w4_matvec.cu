@@ -126,6 +126,12 @@ struct Num {
     static constexpr uint32_t kMagic = F16 ? 0x64006400u : 0x43004300u;
     static constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
     static __device__ __forceinline__ uint32_t bias(uint32_t z) { return (z * 0x10001u) | kMagic | 0x80008000u; }
+    // (v & mask) | magic in one instruction
+    static __device__ __forceinline__ uint32_t nibbles(uint32_t v) {
+        uint32_t d;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(v), "r"(0x000f000fu), "r"(kMagic));
+        return d;
+    }
     static __device__ __forceinline__ uint32_t centred(uint32_t v, uint32_t bias) {
         uint32_t d;
         if (F16)
@@ -165,73 +171,78 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
     return v;
 }
 
-// kWarps warps; `split` warps (a power of two up to kWarps) share a row tile,
-// each with a range of its chunks, and join their sums through shared memory.
-// MT: tiles of 8 activation rows.  Rows past M repeat the last one: columns of
-// the product are independent and theirs are not stored.
-template <bool F16, int MT, bool ZP, int GROUP>
+// kWarps warps; `split` warps (a power of two up to kWarps) share TILES row
+// tiles, each with a range of their chunks, and join their sums through shared
+// memory.  MT: tiles of 8 activation rows.  Rows past M repeat the last one:
+// columns of the product are independent and theirs are not stored.
+template <bool F16, int MT, bool ZP, int GROUP, int TILES>
 __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
-    constexpr int kAhead = 4;                              // chunks in flight
     constexpr int kRuns = GROUP == 32 ? 2 : 1;             // groups in a chunk
     constexpr int kSpan = GROUP < 64 ? 1 : GROUP / 64;     // chunks of a group
+    // Chunks in flight.  Registers, and with them warps, count for more than depth where a warp
+    // holds two tiles of rows or of N: 2 against 4 took 76 us against 85 for 8 rows of the head.
+    constexpr int kAhead = (MT * TILES > 1 || GROUP == 32) && kSpan <= 2 ? 2 : 4;
     constexpr int kMeta = kAhead / kSpan;                  // scales in flight, per run
-    __shared__ float joined[kWarps][16][8 * MT + 1];
+    __shared__ float joined[kWarps][TILES][16][8 * MT + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
     const int part = warp & (a.split - 1);
-    const int per_cta = kWarps / a.split;
-    const int row_tile = blockIdx.x * per_cta + warp / a.split;
+    const int per_cta = kWarps / a.split;  // warps of different row tiles
+    const int row_tile = (blockIdx.x * per_cta + warp / a.split) * TILES, row_tiles = (a.N + 15) / 16;
     const int first = part * a.per_warp;
-    int left = row_tile < (a.N + 15) / 16 ? min(a.per_warp, a.chunks - first) : 0;
-    float acc[MT][4];
+    int left = row_tile < row_tiles ? min(a.per_warp, a.chunks - first) : 0;
+    float acc[TILES][MT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int q = 0; q < TILES; ++q)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[q][i][j] = 0.f;
 
     if (left > 0) {
-        const uint4* tile = a.tiles + (size_t(row_tile) * a.chunks + first) * 32 + lane;
-        const size_t meta = (size_t(row_tile) * a.groups + first / kSpan * kRuns) * 8 + r;
-        const uint32_t* scale = a.scales + meta;
-        const uint8_t* zero = ZP ? a.zeros + meta : nullptr;
+        const uint4* tile[TILES];
+        const uint32_t* scale[TILES];
+        const uint8_t* zero[TILES];
+#pragma unroll
+        for (int q = 0; q < TILES; ++q) {
+            const int of = min(row_tile + q, row_tiles - 1);  // an odd last tile is computed twice, stored once
+            tile[q] = a.tiles + (size_t(of) * a.chunks + first) * 32 + lane;
+            const size_t meta = (size_t(of) * a.groups + first / kSpan * kRuns) * 8 + r;
+            scale[q] = a.scales + meta;
+            zero[q] = ZP ? a.zeros + meta : nullptr;
+        }
         const uint16_t* x[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
             x[i] = static_cast<const uint16_t*>(a.x) + min(8 * i + r, a.M - 1) * a.x_stride + 64 * first + 8 * t;
         // a K of 32 more than a multiple of 64 ends in half a chunk, without the second group
         int halves = GROUP == 32 ? a.K / 32 - 2 * first : 0;
-        uint4 code[kAhead];
-        uint32_t sc[kMeta][kRuns], zp[kMeta][kRuns];
+        uint4 code[TILES][kAhead];
+        uint32_t sc[TILES][kMeta][kRuns], zp[TILES][kMeta][kRuns];
         // chunk d of the next kAhead, `at` chunks further on; the first chunk of a group brings its scale
         auto fetch = [&](int d, int at) {
-            code[d] = load_stream(tile + (at + d) * 32);
+#pragma unroll
+            for (int q = 0; q < TILES; ++q) code[q][d] = load_stream(tile[q] + (at + d) * 32);
             if (d % kSpan == 0) {
 #pragma unroll
                 for (int h = 0; h < kRuns; ++h)
                     if (h == 0 || halves > 2 * (at + d) + h) {
                         const int g = (at + d) / kSpan * kRuns + h;
-                        sc[d / kSpan][h] = __ldg(scale + g * 8);
-                        if (ZP) zp[d / kSpan][h] = __ldg(zero + g * 8);
+#pragma unroll
+                        for (int q = 0; q < TILES; ++q) {
+                            sc[q][d / kSpan][h] = __ldg(scale[q] + g * 8);
+                            if (ZP) zp[q][d / kSpan][h] = __ldg(zero[q] + g * 8);
+                        }
                     }
             }
         };
 #pragma unroll
         for (int d = 0; d < kAhead; ++d)
             if (d < left) fetch(d, 0);
-        float run[MT][4];
+        float run[TILES][MT][4];
         while (left > 0) {
 #pragma unroll
             for (int d = 0; d < kAhead; ++d) {
                 if (d >= left) break;
-                const uint32_t word[4] = {code[d].x, code[d].y, code[d].z, code[d].w};
-                uint32_t s2[kRuns];
-                uint32_t bias_lo[kRuns], bias_hi[kRuns];
-#pragma unroll
-                for (int h = 0; h < kRuns; ++h) {
-                    s2[h] = sc[d / kSpan][h];
-                    const uint32_t z = ZP ? zp[d / kSpan][h] : 0x88u;
-                    bias_lo[h] = Num<F16>::bias(z & 15u), bias_hi[h] = Num<F16>::bias(z >> 4);
-                }
-                // the group's scale is still needed by its later chunks: fetch after its last
                 uint4 b[2][MT];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -239,6 +250,19 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
                     for (int i = 0; i < MT; ++i)
                         if (h == 0 || GROUP != 32 || halves > 2 * d + h)
                             b[h][i] = __ldg(reinterpret_cast<const uint4*>(x[i] + 64 * d + 32 * h));
+                uint4 word[TILES];
+                uint32_t s2[TILES][kRuns], bias[TILES][kRuns][2];
+#pragma unroll
+                for (int q = 0; q < TILES; ++q) {
+                    word[q] = code[q][d];
+#pragma unroll
+                    for (int h = 0; h < kRuns; ++h) {
+                        s2[q][h] = sc[q][d / kSpan][h];
+                        const uint32_t z = ZP ? zp[q][d / kSpan][h] : 0x88u;
+                        bias[q][h][0] = Num<F16>::bias(z & 15u), bias[q][h][1] = Num<F16>::bias(z >> 4);
+                    }
+                }
+                // the group's scale is still needed by its later chunks: fetch after its last
                 if (d % kSpan == kSpan - 1) {
 #pragma unroll
                     for (int e = d - kSpan + 1; e <= d; ++e)
@@ -249,49 +273,62 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
                     if (GROUP == 32 && h == 1 && halves <= 2 * d + 1) break;  // the same for the whole warp
                     const int g = kRuns == 2 ? h : 0;
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        uint32_t frag[4];
+                    for (int p = 0; p < 2; ++p)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            frag[j] = Num<F16>::centred(((word[2 * h + p] >> (4 * j)) & 0x000f000fu) | Num<F16>::kMagic,
-                                                        j & 1 ? bias_hi[g] : bias_lo[g]);
-                        const bool opens = p == 0 && (kRuns == 2 || (h == 0 && d % kSpan == 0));
+                        for (int q = 0; q < TILES; ++q) {
+                            const uint32_t w = h ? (p ? word[q].w : word[q].z) : (p ? word[q].y : word[q].x);
+                            uint32_t frag[4];
 #pragma unroll
-                        for (int i = 0; i < MT; ++i)
-                            Num<F16>::mma(run[i], frag, p ? b[h][i].z : b[h][i].x, p ? b[h][i].w : b[h][i].y, opens);
-                    }
+                            for (int j = 0; j < 4; ++j)
+                                frag[j] = Num<F16>::centred(Num<F16>::nibbles(w >> (4 * j)), bias[q][g][j & 1]);
+                            const bool opens = p == 0 && (kRuns == 2 || (h == 0 && d % kSpan == 0));
+#pragma unroll
+                            for (int i = 0; i < MT; ++i)
+                                Num<F16>::mma(run[q][i], frag, p ? b[h][i].z : b[h][i].x, p ? b[h][i].w : b[h][i].y,
+                                              opens);
+                        }
                     if (kRuns == 2 || (h == 1 && d % kSpan == kSpan - 1)) {
-                        const float lo = scale_value(s2[g] & 0xffffu, a.scale_f16);
-                        const float hi = scale_value(s2[g] >> 16, a.scale_f16);
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            acc[i][0] = __fmaf_rn(lo, run[i][0], acc[i][0]);
-                            acc[i][1] = __fmaf_rn(lo, run[i][1], acc[i][1]);
-                            acc[i][2] = __fmaf_rn(hi, run[i][2], acc[i][2]);
-                            acc[i][3] = __fmaf_rn(hi, run[i][3], acc[i][3]);
+                        for (int q = 0; q < TILES; ++q) {
+                            const float lo = scale_value(s2[q][g] & 0xffffu, a.scale_f16);
+                            const float hi = scale_value(s2[q][g] >> 16, a.scale_f16);
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) {
+                                acc[q][i][0] = __fmaf_rn(lo, run[q][i][0], acc[q][i][0]);
+                                acc[q][i][1] = __fmaf_rn(lo, run[q][i][1], acc[q][i][1]);
+                                acc[q][i][2] = __fmaf_rn(hi, run[q][i][2], acc[q][i][2]);
+                                acc[q][i][3] = __fmaf_rn(hi, run[q][i][3], acc[q][i][3]);
+                            }
                         }
                     }
                 }
             }
             left -= kAhead, halves -= 2 * kAhead;
-            tile += kAhead * 32, scale += kMeta * kRuns * 8;
-            if (ZP) zero += kMeta * kRuns * 8;
+#pragma unroll
+            for (int q = 0; q < TILES; ++q) {
+                tile[q] += kAhead * 32, scale[q] += kMeta * kRuns * 8;
+                if (ZP) zero[q] += kMeta * kRuns * 8;
+            }
 #pragma unroll
             for (int i = 0; i < MT; ++i) x[i] += kAhead * 64;
         }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int q = 0; q < TILES; ++q)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) joined[warp][r + 8 * (j >> 1)][8 * i + 2 * t + (j & 1)] = acc[i][j];
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                joined[warp][q][r + 8 * (j >> 1)][8 * i + 2 * t + (j & 1)] = acc[q][i][j];
     __syncthreads();
     uint32_t fault = 0;
-    const int rows = 16 * per_cta;  // rows of N of this CTA
+    const int rows = 16 * TILES * per_cta;  // rows of N of this CTA
     for (int i = threadIdx.x; i < rows * a.M; i += kWarps * 32) {
         const int m = i / rows, row = i % rows, n = blockIdx.x * rows + row;
         if (n >= a.N) continue;
         float v = 0.f;
-        for (int p = 0; p < a.split; ++p) v = __fadd_rn(v, joined[(row >> 4) * a.split + p][row & 15][m]);
+        for (int p = 0; p < a.split; ++p)
+            v = __fadd_rn(v, joined[row / (16 * TILES) * a.split + p][row / 16 % TILES][row & 15][m]);
         if (!isfinite(v)) fault |= kFlagProjection;
         const size_t at = size_t(m) * a.N + n;
         if (a.out_f32) {
@@ -309,12 +346,12 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
     if (fault) atomicOr(a.flags, fault);
 }
 
-template <bool F16, int MT, bool ZP>
+template <bool F16, int MT, bool ZP, int TILES>
 void launch(const Args& a, int group, int blocks, cudaStream_t stream) {
-    auto* kernel = group == 32    ? w4_matvec_kernel<F16, MT, ZP, 32>
-                   : group == 64  ? w4_matvec_kernel<F16, MT, ZP, 64>
-                   : group == 128 ? w4_matvec_kernel<F16, MT, ZP, 128>
-                                  : w4_matvec_kernel<F16, MT, ZP, 256>;
+    auto* kernel = group == 32    ? w4_matvec_kernel<F16, MT, ZP, 32, TILES>
+                   : group == 64  ? w4_matvec_kernel<F16, MT, ZP, 64, TILES>
+                   : group == 128 ? w4_matvec_kernel<F16, MT, ZP, 128, TILES>
+                                  : w4_matvec_kernel<F16, MT, ZP, 256, TILES>;
     kernel<<<blocks, kWarps * 32, 0, stream>>>(a);
 }
 
@@ -381,18 +418,21 @@ extern "C" cudaError_t ornith_moe_b200_w4_launch(const void* x, int64_t x_stride
     a.out = out, a.flags = static_cast<uint32_t*>(flags);
     a.M = M, a.N = N, a.K = K, a.chunks = k_chunks(K), a.groups = groups;
     a.out_f32 = out_type == 2, a.scale_f16 = scale_type;
-    // Warps that share a row tile: as few as keep 16 warps on each SM.
     const int span = group < 64 ? 1 : group / 64, units = (a.chunks + span - 1) / span;
+    // Row tiles of a warp: two share its activations where that leaves 16 warps on each SM.
+    const int tiles_each = row_tiles(N) >= 2 * kSms * 16 ? 2 : 1, sets = (row_tiles(N) + tiles_each - 1) / tiles_each;
+    // Warps that share row tiles: as few as keep 16 warps on each SM.
     a.split = 1;
-    while (a.split < kWarps && a.split < units && row_tiles(N) * a.split < kSms * 16) a.split *= 2;
+    while (a.split < kWarps && a.split < units && sets * a.split < kSms * 16) a.split *= 2;
     a.per_warp = (units + a.split - 1) / a.split * span;
-    const int per_cta = kWarps / a.split, blocks = (row_tiles(N) + per_cta - 1) / per_cta;
+    const int per_cta = kWarps / a.split, blocks = (sets + per_cta - 1) / per_cta;
     count_launches(1);
     using Launch = void (*)(const Args&, int, int, cudaStream_t);
-    static constexpr Launch table[2][2][2] = {{{launch<false, 1, false>, launch<false, 1, true>},
-                                               {launch<false, 2, false>, launch<false, 2, true>}},
-                                              {{launch<true, 1, false>, launch<true, 1, true>},
-                                               {launch<true, 2, false>, launch<true, 2, true>}}};
-    table[x_type][M > 8][tile_zeros != nullptr](a, group, blocks, stream);
+#define ORNITH_W4(F16, MT) \
+    {{launch<F16, MT, false, 1>, launch<F16, MT, false, 2>}, {launch<F16, MT, true, 1>, launch<F16, MT, true, 2>}}
+    static constexpr Launch table[2][2][2][2] = {{ORNITH_W4(false, 1), ORNITH_W4(false, 2)},
+                                                 {ORNITH_W4(true, 1), ORNITH_W4(true, 2)}};
+#undef ORNITH_W4
+    table[x_type][M > 8][tile_zeros != nullptr][tiles_each - 1](a, group, blocks, stream);
     return cudaGetLastError();
 }
