@@ -737,6 +737,7 @@ def head_launch(x, codes, scales, workspace, out, flags, n, capacity=HEAD_ROWS, 
 # ---------------------------------------------------------------------------
 W4_ROWS, W4_GROUPS, W4_MAX_K, W4_MAX_N = 16, (32, 64, 128, 256), 16384, 1 << 22
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_W4_TYPES = (torch.bfloat16, torch.float16)
 
 
 def w4_pack_shapes(n, k, group):
@@ -757,7 +758,7 @@ def w4_pack(codes, scales, zeros=None):
     Reads the scales and zero points back to check them, so it is not for
     stream capture."""
     if (codes.dtype != torch.uint32 or codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0]
-            or scales.dtype not in (torch.bfloat16, torch.float16) or codes.device.type != 'cuda'
+            or scales.dtype not in _W4_TYPES or codes.device.type != 'cuda'
             or scales.device != codes.device or not codes.is_contiguous() or not scales.is_contiguous()):
         raise ValueError('w4_pack takes contiguous CUDA uint32 codes [N, K/8] and bf16 or fp16 scales [N, K/group]')
     n, k, groups = codes.shape[0], codes.shape[1] * 8, scales.shape[1]
@@ -778,14 +779,27 @@ def w4_pack(codes, scales, zeros=None):
     return tiles, tile_scales, tile_zeros
 
 
-def _launch_on(device, fn, *args):
-    """fn(*args, current stream of `device`) with that device current: the
-    caller's current device may be another one."""
-    index = device.index
+def _launch_on(index, fn, *args):
+    """fn(*args, current stream of device `index`) with that device current:
+    the caller's current device may be another one.  The raw stream query costs
+    a small part of torch.cuda.current_stream, which makes an object; calls of
+    this size are bound by the host."""
     if index == torch.cuda.current_device():
-        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
-        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _w4_bank_fits(tiles, scales, zeros, n, k, index):
+    """Whether (tiles, scales, zeros) is what w4_pack returns for [n, k] on that device."""
+    if scales.dim() != 3 or not scales.shape[1] or k % scales.shape[1] or scales.dtype not in _W4_TYPES:
+        return False
+    tile_shape, scale_shape, zero_shape = w4_pack_shapes(n, k, k // scales.shape[1])
+    return (tiles.shape == tile_shape and tiles.dtype is torch.uint32 and scales.shape == scale_shape
+            and tiles.get_device() == index and scales.get_device() == index and tiles.is_contiguous()
+            and scales.is_contiguous()
+            and (zeros is None or (zeros.shape == zero_shape and zeros.dtype is torch.uint8
+                                   and zeros.get_device() == index and zeros.is_contiguous())))
 
 
 def w4_launch(x, tiles, scales, zeros, out, flags, n, k):
@@ -794,35 +808,27 @@ def w4_launch(x, tiles, scales, zeros, out, flags, n, k):
     x may have rows further apart than k (a multiple of 8 values, rows on 16
     bytes).  flags receives the dense bits 4 (non-finite result) and 8
     (non-finite stored value)."""
-    device = x.device
-    if (x.dim() != 2 or x.shape[1] != k or x.shape[0] > W4_ROWS or x.dtype not in (torch.bfloat16, torch.float16)
-            or device.type != 'cuda' or x.stride(1) != 1):
+    index = x.get_device()
+    if (x.dim() != 2 or x.shape[1] != k or x.shape[0] > W4_ROWS or x.dtype not in _W4_TYPES or index < 0
+            or x.stride(1) != 1):
         raise ValueError(f'w4_launch takes CUDA bf16 or fp16 rows [M <= {W4_ROWS}, {k}]')
-    m, stride = x.shape[0], x.stride(0)
-    if m and (x.data_ptr() % 16 or (m > 1 and (stride < k or stride % 8))):
+    m, stride, at = x.shape[0], x.stride(0), x.data_ptr()
+    if at % 16 or (m > 1 and (stride < k or stride % 8)):
         raise ValueError('w4_launch takes rows that start on 16 bytes and do not overlap')
-    if (out.shape != (m, n) or (out.dtype != x.dtype and out.dtype != torch.float32) or out.device != device
-            or not out.is_contiguous()):
+    if (out.shape != (m, n) or (out.dtype is not x.dtype and out.dtype is not torch.float32)
+            or out.get_device() != index or not out.is_contiguous()):
         raise ValueError(f'w4_launch writes a contiguous [M, {n}] of the type of x or fp32 on the device of x')
-    groups = scales.shape[1] if scales.dim() == 3 else 0
-    if not groups or k % groups:
-        raise ValueError('w4_launch takes the scales that w4_pack returned')
-    tile_shape, scale_shape, zero_shape = w4_pack_shapes(n, k, k // groups)
-    if (tiles.shape != tile_shape or tiles.dtype != torch.uint32 or scales.shape != scale_shape
-            or scales.dtype not in (torch.bfloat16, torch.float16) or tiles.device != device
-            or scales.device != device or not tiles.is_contiguous() or not scales.is_contiguous()
-            or (zeros is not None and (zeros.shape != zero_shape or zeros.dtype != torch.uint8
-                                       or zeros.device != device or not zeros.is_contiguous()))):
+    if not _w4_bank_fits(tiles, scales, zeros, n, k, index):
         raise ValueError(f'w4_launch takes tiles, scales and zero points as w4_pack returns them for [{n}, {k}]')
-    _check_flags(flags, device)
-    check(_launch_on(device, lib().ornith_moe_b200_w4_launch, x.data_ptr(), stride, _TYPES[x.dtype],
-                     tiles.data_ptr(), scales.data_ptr(), _TYPES[scales.dtype],
-                     None if zeros is None else zeros.data_ptr(), out.data_ptr(), _TYPES[out.dtype],
-                     flags.data_ptr(), m, n, k, k // groups), 'W4 product')
+    _check_flags(flags, index)
+    check(_launch_on(index, lib().ornith_moe_b200_w4_launch, at, stride, _TYPES[x.dtype], tiles.data_ptr(),
+                     scales.data_ptr(), _TYPES[scales.dtype], None if zeros is None else zeros.data_ptr(),
+                     out.data_ptr(), _TYPES[out.dtype], flags.data_ptr(), m, n, k, k // scales.shape[1]),
+          'W4 product')
 
 
-def _check_flags(flags, device):
-    if flags.dtype != torch.int32 or flags.numel() != 1 or flags.device != device:
+def _check_flags(flags, index):
+    if flags.dtype is not torch.int32 or flags.numel() != 1 or flags.get_device() != index:
         raise ValueError('flags is one int32 word on the device of the input')
 
 
@@ -864,9 +870,8 @@ def sample_launch(logits, temperature, top_k, top_p, min_p, uniform, tokens, log
     raises a bit of flags: 1 NaN or +inf among its logits, 2 a parameter out of
     range (temperature outside [0, 1e30], negative top_p, min_p outside [0, 1],
     uniform outside [0, 1), any NaN), 4 every logit -inf."""
-    device = logits.device
-    if (logits.dim() != 2 or logits.dtype not in _TYPES or device.type != 'cuda'
-            or not 0 < logits.shape[1] <= SAMPLE_MAX_VOCAB
+    index = logits.get_device()
+    if (logits.dim() != 2 or logits.dtype not in _TYPES or index < 0 or not 0 < logits.shape[1] <= SAMPLE_MAX_VOCAB
             or (logits.shape[1] > 1 and logits.stride(1) != 1)):
         raise ValueError(f'sample_launch takes CUDA bf16, fp16 or fp32 logits [M, V <= {SAMPLE_MAX_VOCAB}] with '
                          'neighbouring values')
@@ -874,21 +879,25 @@ def sample_launch(logits, temperature, top_k, top_p, min_p, uniform, tokens, log
     stride = logits.stride(0) if m > 1 else vocab
     if stride < vocab:
         raise ValueError('sample_launch takes rows that do not overlap')
-    for name, t, dtype, optional in (('temperature', temperature, torch.float32, True),
-                                     ('top_k', top_k, torch.int32, True), ('top_p', top_p, torch.float32, True),
-                                     ('min_p', min_p, torch.float32, True),
-                                     ('uniform', uniform, torch.float32, False),
-                                     ('tokens', tokens, torch.int32, False),
-                                     ('logprobs', logprobs, torch.float32, True)):
-        if t is None and optional:
-            continue
-        if t is None or t.dtype != dtype or t.shape != (m,) or t.device != device or not t.is_contiguous():
-            raise ValueError(f'sample_launch takes {name} as a contiguous {dtype} [{m}] on the device of the logits')
-    _check_flags(flags, device)
-    check(_launch_on(device, lib().ornith_moe_b200_sample_launch, logits.data_ptr(), stride, _TYPES[logits.dtype],
-                     *[None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p, uniform,
-                                                                     tokens, logprobs, flags)],
-                     m, vocab), 'sampling')
+    rows = [_row_pointer(t, name, dtype, m, index) for t, name, dtype in (
+        (temperature, 'temperature', torch.float32), (top_k, 'top_k', torch.int32), (top_p, 'top_p', torch.float32),
+        (min_p, 'min_p', torch.float32), (uniform, 'uniform', torch.float32), (tokens, 'tokens', torch.int32),
+        (logprobs, 'logprobs', torch.float32))]
+    if uniform is None or tokens is None:
+        raise ValueError('sample_launch needs uniform and tokens')
+    _check_flags(flags, index)
+    check(_launch_on(index, lib().ornith_moe_b200_sample_launch, logits.data_ptr(), stride, _TYPES[logits.dtype],
+                     *rows, flags.data_ptr(), m, vocab), 'sampling')
+
+
+def _row_pointer(t, name, dtype, rows, index):
+    """The address of a row parameter, None for one that is not given."""
+    if t is None:
+        return None
+    if (t.dtype is not dtype or t.dim() != 1 or t.shape[0] != rows or t.get_device() != index
+            or not t.is_contiguous()):
+        raise ValueError(f'sample_launch takes {name} as a contiguous {dtype} [{rows}] on the device of the logits')
+    return t.data_ptr()
 
 
 @torch.library.custom_op('ornith_b200::sample_out', mutates_args={'tokens', 'logprobs', 'flags'},
