@@ -21,11 +21,16 @@
 //
 // Layout of the work.  A cluster of 1 to 16 CTAs takes one row: every CTA
 // keeps its share of the logits in shared memory, so the row is read from HBM
-// once, however many steps the selection takes.  A cut (top-k or top-p) is
-// found by histograms over the value range, merged through distributed shared
-// memory; the bin that holds the border is ranked exactly when it has few
-// tokens, split again when it has many, and resolved by index when all its
-// logits are equal.
+// once, however many steps the selection takes.  While the logits come in, a
+// CTA counts them by their leading 16 bits (a bf16's own value); the merged
+// counts say where a cut lies.  From there:
+//   - a bf16 row is known but for its order: masses are counts times weights,
+//     a cut is a value and a number of equal logits;
+//   - for fp16 and fp32 the counts bound the masses, and only the tokens of the
+//     bins that can hold the border are looked at one by one;
+//   - where at most 256 tokens can be kept, one CTA ranks and draws among them;
+//     else each CTA weighs its kept tokens and the one that holds the drawn
+//     token finds it.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -112,7 +117,7 @@ struct Pair {
     u64 a, b;
 };
 
-// The search of a cut by value ranges.
+// The search of a cut among the values of a range (cut_row).
 struct Search {
     u64 mass[kBins], tmass[kBins];       // this CTA's histogram, the row's
     uint32_t cnt[kBins], tcnt[kBins];
@@ -122,16 +127,48 @@ struct Search {
     uint32_t ln;
 };
 
-// The value histogram of a bf16 row (see value_row).
-constexpr int kCodes = 19 * 128;                              // magnitudes from 2^-12 up to 128
-constexpr int kTinyBin = kCodes, kValueBins = 2 * kCodes + 1;  // by value, largest first; zero and below 2^-12 between
-constexpr int kPerThread = (kValueBins + kThreads - 1) / kThreads, kTinyCap = 64;
+// Counts of the logits' leading 16 bits: 4352 codes of magnitude 2^-10 to 128,
+// and all below 2^-10 as one.
+constexpr int kOctaves = 17, kCodes = kOctaves * 128;
+constexpr uint32_t kFirstCode = (134 - kOctaves) << 7;         // of 2^-10
+constexpr int kTinyBin = kCodes, kValueBins = 2 * kCodes + 1;  // by value, largest first; the tiny between
+constexpr int kPerThread = (kValueBins + kThreads - 1) / kThreads, kTinyCap = 256;
 struct Values {
     uint32_t own[kValueBins];                      // by code: positive, negative, tiny
     uint32_t all[kPerThread * kThreads];           // the row's, by value
-    float tiny[kTinyCap];                          // this CTA's tiny logits
+    float tiny[kTinyCap];                          // this CTA's tiny logits (bf16 rows)
     u64 tiny_mass[kMaxCluster];                    // pushed
-    uint32_t tiny_n;
+};
+
+// A bin's largest and smallest value; the same for bf16 but in the tiny one.
+__device__ __forceinline__ int code_of(int bin) {
+    return bin < kTinyBin ? kCodes - 1 - bin : bin == kTinyBin ? 2 * kCodes : bin - 1;
+}
+__device__ __forceinline__ uint32_t magnitude_of(int bin) {
+    return (uint32_t(bin < kTinyBin ? kCodes - 1 - bin : bin - 1 - kCodes) + kFirstCode) << 16;
+}
+__device__ __forceinline__ float near_edge(int bin) {  // the edge next to zero
+    if (bin == kTinyBin) return 0.f;
+    return __uint_as_float(magnitude_of(bin) | (bin < kTinyBin ? 0u : 0x80000000u));
+}
+__device__ __forceinline__ float far_edge(int bin) {
+    return __uint_as_float(__float_as_uint(near_edge(bin)) | 0xffffu);
+}
+__device__ __forceinline__ float bin_top(int bin) {
+    if (bin == kTinyBin) return __uint_as_float((kFirstCode << 16) - 1);
+    return bin < kTinyBin ? far_edge(bin) : near_edge(bin);
+}
+__device__ __forceinline__ float bin_bottom(int bin) {
+    if (bin == kTinyBin) return -__uint_as_float((kFirstCode << 16) - 1);
+    return bin < kTinyBin ? near_edge(bin) : far_edge(bin);
+}
+
+// The tokens that can be kept, where they are few: pushed to the first CTA.
+struct List {
+    u64 weight[kCap];                    // by rank
+    float v[kCap], ranked_v[kCap];
+    int i[kCap], ranked_i[kCap];
+    uint32_t n;
 };
 
 struct Shared {
@@ -139,6 +176,7 @@ struct Shared {
         Search search;
         Values values;
     };
+    List list;
     double pow64[64];                    // 2^(-j/64)
     Pair slot[2][kMaxCluster];           // pushed by every CTA of the cluster in turn
     u64 slab[kSlabs];                    // kept mass of each (turn, warp) in index order
@@ -249,118 +287,90 @@ __device__ __forceinline__ u64 block_exclusive(Shared& sh, u64 v) {
     return before + prior;
 }
 
-// The smallest prefix of the kept tokens, by (value, index), that has `k`
-// tokens (MASS false) or `share` / 2^64 of their mass, becomes the kept set.
+__device__ double block_exclusive_double(Shared& sh, double v) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double inc = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += o;
+    }
+    __syncthreads();
+    if (lane == 31) sh.red[warp].a = u64(__double_as_longlong(inc));
+    __syncthreads();
+    double before = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+        if (w < warp) before += __longlong_as_double(sh.red[w].a);
+    const double prior = __shfl_up_sync(0xffffffffu, inc, 1);
+    return lane ? before + prior : before;
+}
+
+// Tokens in the bins before `bin`, from counts that lie kPerThread to a thread.
+__device__ u64 count_above(Shared& sh, int first, u64 before, const uint32_t (&cnt)[kPerThread], int bin) {
+    __syncthreads();
+    if (first <= bin && bin < first + kPerThread) {
+        u64 c = before;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i)
+            if (first + i < bin) c += cnt[i];
+        sh.bound[0] = c;
+    }
+    __syncthreads();
+    return sh.bound[0];
+}
+
+// (n + d - 1) / d for n < 2^63 and 1 <= d: a quotient in double precision, put right.
+__device__ __forceinline__ u64 ceil_div(u64 n, u64 d) {
+    u64 q = u64(__ddiv_rn(double(n), double(d)));
+    while (q > 0 && (q - 1) * d >= n) --q;
+    while (q * d < n) ++q;
+    return q;
+}
+
+// The index of this CTA's `nth` kept token (from 1) whose logit is `value`; -1
+// where it has fewer.
+template <int TY>
+__device__ int nth_equal(const Row<TY>& r, float value, u64 nth) {
+    const int slots = r.nvec * Elem<TY>::E, per_thread = (slots + kThreads - 1) / kThreads;
+    const int s0 = min(int(threadIdx.x) * per_thread, slots), s1 = min(s0 + per_thread, slots);
+    const auto tie = [&](int slot) {
+        return Elem<TY>::one(reinterpret_cast<const char*>(r.data) + size_t(slot) * Elem<TY>::kBytes) == value &&
+               r.kept(value, slot);
+    };
+    u64 ties = 0;
+    for (int s = s0; s < s1; ++s) ties += tie(s);
+    u64 rankth = block_exclusive(r.sh, ties);
+    if (threadIdx.x == 0) r.sh.found_bin = -1;
+    __syncthreads();
+    if (rankth < nth && nth <= rankth + ties)
+        for (int s = s0; s < s1; ++s)
+            if (tie(s) && ++rankth == nth) r.sh.found_bin = r.first + s;
+    __syncthreads();
+    return r.sh.found_bin;
+}
+
+// Cuts the kept set inside [lo, hi], which holds at most `n` of it: `base`
+// tokens (mass, where MASS) lie above, and the smallest prefix by (value,
+// index) with `target` stays.  Where there is no such prefix nothing is cut.
 // Every CTA of the cluster takes the same decisions from the same merged sums.
 template <int TY, bool MASS>
-__device__ void cut_row(Row<TY>& r, float low, u64 k, u64 share) {
+__device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u64 n) {
     Shared& sh = r.sh;
+    Search& f = sh.search;
     auto cluster = cg::this_cluster();
     const int per = kBins / r.size;  // bins that one CTA merges
-    float hi = r.top, lo = low;
-    u64 base = 0, target = k;
-    for (bool first_level = true;; first_level = false) {
-        const float scale = __fdiv_rn(float(kBins), __fsub_rn(hi, lo));
-        auto bin = [&](float x) { return max(0, min(kBins - 1, __float2int_rz(__fmul_rn(__fsub_rn(hi, x), scale)))); };
-        for (int b = threadIdx.x; b < kBins; b += kThreads) {
-            sh.search.cnt[b] = 0;
-            if (MASS) sh.search.mass[b] = 0;
-        }
-        if (threadIdx.x == 0) sh.found = 0;
-        __syncthreads();
-        r.each([&](float x, int slot) {
-            if (x >= lo && x <= hi && r.kept(x, slot)) {
-                const int b = bin(x);
-                atomicAdd(&sh.search.cnt[b], 1u);
-                if (MASS) atomicAdd(&sh.search.mass[b], r.weight(x));
-            }
-        });
-        cluster.sync();  // also: nobody reads the list of a search before this one any more
-        if (threadIdx.x == 0) sh.search.ln = 0;
-        for (int i = threadIdx.x; i < per; i += kThreads) {
-            const int b = r.rank * per + i;
-            uint32_t c = 0;
-            u64 w = 0;
-            for (int q = 0; q < r.size; ++q) {
-                c += *cluster.map_shared_rank(&sh.search.cnt[b], q);
-                if (MASS) w += *cluster.map_shared_rank(&sh.search.mass[b], q);
-            }
-            for (int q = 0; q < r.size; ++q) {
-                *cluster.map_shared_rank(&sh.search.tcnt[b], q) = c;
-                if (MASS) *cluster.map_shared_rank(&sh.search.tmass[b], q) = w;
-            }
-        }
-        cluster.sync();
-        // two bins a thread, from the largest values down
-        const int b0 = 2 * threadIdx.x;
-        const u64 v0 = MASS ? sh.search.tmass[b0] : sh.search.tcnt[b0], v1 = MASS ? sh.search.tmass[b0 + 1] : sh.search.tcnt[b0 + 1];
-        const u64 before = block_exclusive(sh, v0 + v1);
-        if (first_level) {
-            if (threadIdx.x == kThreads - 1) sh.bound[0] = before + v0 + v1;
-            __syncthreads();
-            const u64 total = sh.bound[0];
-            if (MASS)
-                target = max(u64(1), __umul64hi(total, share) + (total * share != 0));
-            else if (total <= target)
-                return;
-        }
-        const u64 at = base + before;
-        if (at < target && target <= at + v0) sh.found_bin = b0, sh.bound[1] = at, sh.found = 1;
-        if (at + v0 < target && target <= at + v0 + v1) sh.found_bin = b0 + 1, sh.bound[1] = at + v0, sh.found = 1;
-        __syncthreads();
-        if (!sh.found) return;  // no mass at all: nothing to cut
-        const int border = sh.found_bin;
-        const uint32_t n = sh.search.tcnt[border];
-        base = sh.bound[1];
-        if (n <= uint32_t(kCap)) {
-            // rank the border's tokens exactly
-            r.each([&](float x, int slot) {
-                if (x >= lo && x <= hi && r.kept(x, slot) && bin(x) == border) {
-                    const uint32_t at_list = atomicAdd(&sh.search.ln, 1u);
-                    if (at_list < uint32_t(kCap)) sh.search.lv[at_list] = x, sh.search.li[at_list] = r.first + slot;
-                }
-            });
-            cluster.sync();
-            // every CTA's count, then each thread one candidate of the row
-            if (int(threadIdx.x) < r.size)
-                sh.slab[threadIdx.x] = *cluster.map_shared_rank(&sh.search.ln, threadIdx.x);
-            __syncthreads();
-            int from = 0, owner = -1, at_owner = 0;
-            for (int q = 0; q < r.size; ++q) {
-                const int m = min(int(sh.slab[q]), kCap - from);
-                if (int(threadIdx.x) >= from && int(threadIdx.x) < from + m) owner = q, at_owner = threadIdx.x - from;
-                from += m;
-            }
-            if (owner >= 0) {
-                sh.search.gv[threadIdx.x] = *cluster.map_shared_rank(&sh.search.lv[at_owner], owner);
-                sh.search.gi[threadIdx.x] = *cluster.map_shared_rank(&sh.search.li[at_owner], owner);
-            }
-            __syncthreads();
-            int place = 0;
-            float x = 0.f;
-            int index = 0;
-            const bool mine = int(threadIdx.x) < from;
-            if (mine) {
-                x = sh.search.gv[threadIdx.x], index = sh.search.gi[threadIdx.x];
-                for (int j = 0; j < from; ++j) place += sh.search.gv[j] > x || (sh.search.gv[j] == x && sh.search.gi[j] < index);
-                sh.search.gw[place] = MASS ? r.weight(x) : 1;
-            }
-            __syncthreads();
-            const u64 w = int(threadIdx.x) < from ? sh.search.gw[threadIdx.x] : 0;
-            const u64 sum = base + block_exclusive(sh, w);
-            if (sum < target && target <= sum + w) sh.found_bin = threadIdx.x;  // its place
-            __syncthreads();
-            const int last = sh.found_bin;
-            if (mine && place == last) sh.bound[0] = as_bits(x), sh.bound[1] = u64(uint32_t(index));
-            __syncthreads();
-            r.cut_v = as_float(sh.bound[0]), r.cut_i = int(uint32_t(sh.bound[1]));
-            __syncthreads();
-            return;
-        }
-        // the border's smallest and largest value
+    float scale = 0.f;               // of the last histogram
+    int border = -1;                 // its bin, where there was one
+    auto bin = [&](float x) { return max(0, min(kBins - 1, __float2int_rz(__fmul_rn(__fsub_rn(hi, x), scale)))); };
+    auto inside = [&](float x, int slot) {
+        return x >= lo && x <= hi && r.kept(x, slot) && (border < 0 || bin(x) == border);
+    };
+    while (n > u64(kCap)) {
+        // the values left: all alike, or split
         float mn = INFINITY, mx = -INFINITY;
         r.each([&](float x, int slot) {
-            if (x >= lo && x <= hi && r.kept(x, slot) && bin(x) == border) mn = fminf(mn, x), mx = fmaxf(mx, x);
+            if (inside(x, slot)) mn = fminf(mn, x), mx = fmaxf(mx, x);
         });
         auto range = [](Pair p, Pair q) {
             return Pair{as_bits(fminf(as_float(p.a), as_float(q.a))), as_bits(fmaxf(as_float(p.b), as_float(q.b)))};
@@ -368,41 +378,114 @@ __device__ void cut_row(Row<TY>& r, float low, u64 k, u64 share) {
         Pair own = block_reduce(sh, Pair{as_bits(mn), as_bits(mx)}, range);
         const Pair* all = r.exchange(own);
         for (int q = 0; q < r.size; ++q) own = range(own, all[q]);
-        lo = as_float(own.a), hi = as_float(own.b);
-        if (lo < hi) continue;
-        // equal logits: the lowest indices are kept
-        u64 need = target - base;
-        if (MASS) {
-            const u64 w = r.weight(hi);
-            need = (need + w - 1) / w;
+        lo = as_float(own.a), hi = as_float(own.b), border = -1;
+        if (!(lo < hi)) {
+            if (lo > hi) return;  // none
+            // equal logits: the lowest indices are kept
+            u64 need = target - base;
+            if (MASS) {
+                const u64 w = r.weight(hi);
+                if (w == 0) return;
+                need = ceil_div(need, w);
+            }
+            u64 ties = 0;
+            r.each([&](float x, int slot) { ties += inside(x, slot); });
+            auto add = [](Pair p, Pair q) { return Pair{p.a + q.a, 0}; };
+            all = r.exchange(block_reduce(sh, Pair{ties, 0}, add));
+            u64 ahead = 0;
+            for (int q = 0; q < r.rank; ++q) ahead += all[q].a;
+            const int mine = nth_equal(r, hi, ahead < need ? need - ahead : 0);
+            all = r.exchange(Pair{u64(uint32_t(mine)), 0});
+            int index = -1;
+            for (int q = 0; q < r.size; ++q) index = max(index, int(uint32_t(all[q].a)));
+            if (index >= 0) r.cut_v = hi, r.cut_i = index;
+            return;
         }
-        const int per_thread = (r.nvec * Row<TY>::El::E + kThreads - 1) / kThreads;
-        const int s0 = min(int(threadIdx.x) * per_thread, r.nvec * Row<TY>::El::E);
-        const int s1 = min(s0 + per_thread, r.nvec * Row<TY>::El::E);
-        const auto value = [&](int slot) {
-            return Row<TY>::El::one(reinterpret_cast<const char*>(r.data) + size_t(slot) * Row<TY>::El::kBytes);
-        };
-        u64 ties = 0;
-        for (int s = s0; s < s1; ++s) ties += value(s) == hi && r.kept(hi, s);
-        const u64 prior = block_exclusive(sh, ties);
-        if (threadIdx.x == kThreads - 1) sh.bound[0] = prior + ties;
+        scale = __fdiv_rn(float(kBins), __fsub_rn(hi, lo));
+        for (int b = threadIdx.x; b < kBins; b += kThreads) {
+            f.cnt[b] = 0;
+            if (MASS) f.mass[b] = 0;
+        }
+        if (threadIdx.x == 0) sh.found = 0;
         __syncthreads();
-        all = r.exchange(Pair{sh.bound[0], 0});
-        u64 ahead = 0;
-        for (int q = 0; q < r.rank; ++q) ahead += all[q].a;
-        if (threadIdx.x == 0) sh.found_bin = -1;
+        r.each([&](float x, int slot) {
+            if (inside(x, slot)) {
+                const int b = bin(x);
+                atomicAdd(&f.cnt[b], 1u);
+                if (MASS) atomicAdd(&f.mass[b], r.weight(x));
+            }
+        });
+        cluster.sync();
+        for (int i = threadIdx.x; i < per; i += kThreads) {
+            const int b = r.rank * per + i;
+            uint32_t c = 0;
+            u64 w = 0;
+            for (int q = 0; q < r.size; ++q) {
+                c += *cluster.map_shared_rank(&f.cnt[b], q);
+                if (MASS) w += *cluster.map_shared_rank(&f.mass[b], q);
+            }
+            for (int q = 0; q < r.size; ++q) {
+                *cluster.map_shared_rank(&f.tcnt[b], q) = c;
+                if (MASS) *cluster.map_shared_rank(&f.tmass[b], q) = w;
+            }
+        }
+        cluster.sync();
+        // two bins a thread, from the largest values down
+        const int b0 = 2 * threadIdx.x;
+        const u64 v0 = MASS ? f.tmass[b0] : f.tcnt[b0], v1 = MASS ? f.tmass[b0 + 1] : f.tcnt[b0 + 1];
+        const u64 at = base + block_exclusive(sh, v0 + v1);
+        if (at < target && target <= at + v0) sh.found_bin = b0, sh.bound[1] = at, sh.found = 1;
+        if (at + v0 < target && target <= at + v0 + v1) sh.found_bin = b0 + 1, sh.bound[1] = at + v0, sh.found = 1;
         __syncthreads();
-        u64 rankth = ahead + prior;
-        if (rankth < need && need <= rankth + ties)
-            for (int s = s0; s < s1; ++s)
-                if (value(s) == hi && r.kept(hi, s) && ++rankth == need) sh.found_bin = r.first + s;
-        __syncthreads();
-        all = r.exchange(Pair{u64(uint32_t(sh.found_bin)), 0});
-        int index = -1;
-        for (int q = 0; q < r.size; ++q) index = max(index, int(uint32_t(all[q].a)));
-        r.cut_v = hi, r.cut_i = index;
-        return;
+        if (!sh.found) return;
+        border = sh.found_bin, base = sh.bound[1];
+        n = f.tcnt[border];
+        __syncthreads();  // found is written again
     }
+    // rank the tokens left exactly; the exchange before tells every CTA that nobody reads the lists any more
+    r.exchange(Pair{0, 0});
+    if (threadIdx.x == 0) f.ln = 0, sh.found = 0;
+    __syncthreads();
+    r.each([&](float x, int slot) {
+        if (inside(x, slot)) {
+            const uint32_t at_list = atomicAdd(&f.ln, 1u);
+            if (at_list < uint32_t(kCap)) f.lv[at_list] = x, f.li[at_list] = r.first + slot;
+        }
+    });
+    cluster.sync();
+    // every CTA's count, then each thread one candidate of the row
+    if (int(threadIdx.x) < r.size) sh.slab[threadIdx.x] = *cluster.map_shared_rank(&f.ln, threadIdx.x);
+    __syncthreads();
+    int from = 0, owner = -1, at_owner = 0;
+    for (int q = 0; q < r.size; ++q) {
+        const int m = min(int(sh.slab[q]), kCap - from);
+        if (int(threadIdx.x) >= from && int(threadIdx.x) < from + m) owner = q, at_owner = threadIdx.x - from;
+        from += m;
+    }
+    if (owner >= 0) {
+        f.gv[threadIdx.x] = *cluster.map_shared_rank(&f.lv[at_owner], owner);
+        f.gi[threadIdx.x] = *cluster.map_shared_rank(&f.li[at_owner], owner);
+    }
+    __syncthreads();
+    int place = 0;
+    float x = 0.f;
+    int index = 0;
+    const bool mine = int(threadIdx.x) < from;
+    if (mine) {
+        x = f.gv[threadIdx.x], index = f.gi[threadIdx.x];
+        for (int j = 0; j < from; ++j) place += f.gv[j] > x || (f.gv[j] == x && f.gi[j] < index);
+        f.gw[place] = MASS ? r.weight(x) : 1;
+    }
+    __syncthreads();
+    const u64 w = mine ? f.gw[threadIdx.x] : 0;
+    const u64 sum = base + block_exclusive(sh, w);
+    if (sum < target && target <= sum + w) sh.found_bin = threadIdx.x, sh.found = 1;  // its place
+    __syncthreads();
+    const bool found = sh.found;
+    if (mine && found && place == sh.found_bin) sh.bound[0] = as_bits(x), sh.bound[1] = u64(uint32_t(index));
+    __syncthreads();
+    if (found) r.cut_v = as_float(sh.bound[0]), r.cut_i = int(uint32_t(sh.bound[1]));
+    __syncthreads();
 }
 
 // The kept mass of each (turn, warp) of this CTA into sh.slab, and its sum.
@@ -433,8 +516,10 @@ __device__ u64 slab_masses(const Row<TY>& r, int turns) {
     for (int turn = 0; turn < turns; ++turn) {
         u64 w[Elem<TY>::E];
         u64 sum = vector_mass(r, turn * kThreads + int(threadIdx.x), w);
+        if (__any_sync(0xffffffffu, sum != 0)) {
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        }
         if (lane == 0) r.sh.slab[turn * kWarps + warp] = sum;
         mine += sum;
     }
@@ -444,9 +529,9 @@ __device__ u64 slab_masses(const Row<TY>& r, int turns) {
 // The log probability of a token x: sums of exp(logit - top) over the largest
 // logits (`tops` of them) and the others.
 struct Partition {
-    double tops, others;
+    float tops, others;
     __device__ float of(float x, float top) const {
-        return float((double(x) - double(top)) - (log(tops) + log1p(others / tops)));
+        return float((double(x) - double(top)) - double(__fadd_rn(logf(tops), log1pf(__fdiv_rn(others, tops)))));
     }
 };
 
@@ -487,200 +572,346 @@ __device__ void write_token(const Row<TY>& r, const Args& a, int row, u64 ahead,
     }
 }
 
-__device__ __forceinline__ Pair add_doubles(Pair p, Pair q) {
-    return Pair{u64(__double_as_longlong(__longlong_as_double(p.a) + __longlong_as_double(q.a))),
-                u64(__double_as_longlong(__longlong_as_double(p.b) + __longlong_as_double(q.b)))};
+__device__ __forceinline__ Pair add_floats(Pair p, Pair q) {
+    return Pair{as_bits(__fadd_rn(as_float(p.a), as_float(q.a))), as_bits(__fadd_rn(as_float(p.b), as_float(q.b)))};
+}
+__device__ __forceinline__ Pair add_pairs(Pair p, Pair q) { return Pair{p.a + q.a, p.b + q.b}; }
+
+// floor(u * mass): the token is the first whose running mass is above it.
+__device__ __forceinline__ u64 drawn(u64 mass, float u) { return __umul64hi(mass, __double2ull_rz(double(u) * 0x1p64)); }
+// ceil(p * mass), 1 at least, for p < 1.
+__device__ __forceinline__ u64 nucleus(u64 mass, float p) {
+    const u64 share = __double2ull_rz(double(p) * 0x1p64);
+    return max(u64(1), __umul64hi(mass, share) + (mass * share != 0));
 }
 
-// The index of this CTA's `nth` token (from 1) whose logit is `value`.
+// The largest logits and the others in a bf16 row's counts.
+__device__ Partition partition_of(Row<0>& r) {
+    const Values& h = r.sh.values;
+    float others = 0.f, tops = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+        const int bin = int(threadIdx.x) * kPerThread + i;
+        const float c = float(h.all[bin]);
+        if (c > 0.f) {
+            const float v = near_edge(bin);
+            if (v == r.top)
+                tops = c;
+            else
+                others = __fmaf_rn(c, expf(__fsub_rn(v, r.top)), others);
+        }
+    }
+    const Pair sums = block_reduce(r.sh, Pair{as_bits(tops), as_bits(others)}, add_floats);
+    return Partition{as_float(sums.a), as_float(sums.b)};
+}
+
+// Pushes the tokens at `bottom` or above (kCap at most) to the cluster's first
+// CTA.  The caller synchronises the cluster next.
 template <int TY>
-__device__ int nth_equal(const Row<TY>& r, float value, u64 nth) {
-    const int slots = r.nvec * Elem<TY>::E, per_thread = (slots + kThreads - 1) / kThreads;
-    const int s0 = min(int(threadIdx.x) * per_thread, slots), s1 = min(s0 + per_thread, slots);
-    const auto at = [&](int slot) {
-        return Elem<TY>::one(reinterpret_cast<const char*>(r.data) + size_t(slot) * Elem<TY>::kBytes);
-    };
-    u64 ties = 0;
-    for (int s = s0; s < s1; ++s) ties += at(s) == value;
-    u64 rankth = block_exclusive(r.sh, ties);
-    if (rankth < nth && nth <= rankth + ties)
-        for (int s = s0; s < s1; ++s)
-            if (at(s) == value && ++rankth == nth) r.sh.found_bin = r.first + s;
-    __syncthreads();
-    return r.sh.found_bin;
+__device__ void push_list(const Row<TY>& r, float bottom) {
+    auto cluster = cg::this_cluster();
+    List& l = *cluster.map_shared_rank(&r.sh.list, 0);
+    r.each([&](float x, int slot) {
+        if (x >= bottom) {
+            const uint32_t at = atomicAdd(&l.n, 1u);
+            if (at < uint32_t(kCap)) l.v[at] = x, l.i[at] = r.first + slot;
+        }
+    });
 }
 
-// A bf16 row by its values.  A row of 10^5 logits has a few thousand distinct
-// values, so counts of each value, an exact histogram over the 4864 codes of
-// magnitude 2^-12 to 128, hold everything but the order: masses are counts
-// times weights, a cut is a value and a number of equal logits, and only the
-// CTA that holds the token goes over its logits again.  One shared-memory
-// count a logit replaces a double-precision exponential a logit.  The few
-// logits below 2^-12 are kept in a list and weighted one by one.
-//
-// Returns false, in every CTA alike, where a cut falls among those: the row
-// then goes the general way.
-__device__ bool value_row(Row<0>& r, const Args& a, int row, float T, int k, float p, float u, float floor_v,
-                          bool greedy) {
+// The first CTA ranks its list, applies top-k (`limit`) and top-p and draws.
+// `whole`: the mass that top-p refers to; 0: that of the first `limit`.
+template <int TY>
+__device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 limit, float p, float u, u64 whole,
+                               const Partition& z) {
+    Shared& sh = r.sh;
+    List& l = sh.list;
+    const int tid = threadIdx.x, n = min(int(l.n), kCap);
+    // two threads a token; the order of the list varies, the ranks do not
+    const int e = tid >> 1, half = tid & 1;
+    int rank = 0;
+    float x = 0.f;
+    int index = 0;
+    if (e < n) {
+        x = l.v[e], index = l.i[e];
+        for (int j = half; j < n; j += 2) rank += l.v[j] > x || (l.v[j] == x && l.i[j] < index);
+    }
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    if (e < n && half == 0) l.weight[rank] = u64(rank) < limit ? r.weight(x) : 0, l.ranked_v[rank] = x, l.ranked_i[rank] = index;
+    if (tid == 0) sh.found_bin = int(min(u64(n), limit)) - 1;
+    __syncthreads();
+    u64 w = tid < n ? l.weight[tid] : 0;
+    if (p < 1.f) {
+        const u64 before = block_exclusive(sh, w);
+        if (tid == kThreads - 1) sh.bound[0] = before + w;
+        __syncthreads();
+        const u64 target = nucleus(whole ? whole : sh.bound[0], p);
+        if (before < target && target <= before + w) sh.found_bin = tid;
+        __syncthreads();
+    }
+    const int keep = sh.found_bin + 1;
+    const u64 mass = block_reduce(sh, Pair{tid < keep ? w : 0, 0}, add_pairs).a;
+    const u64 target = drawn(mass, u);
+    // mass up to each kept token in index order
+    w = 0;
+    u64 upto = 0;
+    if (e < keep) {
+        index = l.ranked_i[e], w = l.weight[e];
+        for (int j = half; j < keep; j += 2)
+            if (l.ranked_i[j] <= index) upto += l.weight[j];
+    }
+    upto += __shfl_xor_sync(0xffffffffu, upto, 1);
+    if (half == 0 && upto > target && upto - w <= target) {
+        a.tokens[row] = index;
+        if (a.logprobs) a.logprobs[row] = z.of(l.ranked_v[e], r.top);
+    }
+}
+
+// Kept masses of the CTAs -> the one that holds the token finds it.
+template <int TY>
+__device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, const Partition& z) {
+    const int turns = (a.vecs + kThreads - 1) / kThreads;
+    const Pair own = block_reduce(r.sh, Pair{slab_masses(r, turns), 0}, add_pairs);
+    const Pair* all = r.exchange(own);
+    u64 whole = 0, ahead = 0;
+    for (int q = 0; q < r.size; ++q) {
+        if (q < r.rank) ahead += all[q].a;
+        whole += all[q].a;
+    }
+    const u64 target = drawn(whole, u);
+    if (ahead <= target && target < ahead + own.a && threadIdx.x < 32) write_token(r, a, row, ahead, target, turns, z);
+}
+
+// The row's counts, by value, in every CTA; and for bf16 the mass of the tiny.
+template <int TY>
+__device__ u64 merge_counts(const Row<TY>& r) {
+    Values& h = r.sh.values;
+    auto cluster = cg::this_cluster();
+    const int per = (kValueBins + r.size - 1) / r.size;
+    for (int i = threadIdx.x; i < per; i += kThreads) {
+        const int bin = r.rank * per + i;
+        if (bin >= kValueBins) break;
+        uint32_t c = 0;
+        for (int q = 0; q < r.size; q += 8) {  // eight loads from other CTAs at a time
+            uint32_t part[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                part[j] = q + j < r.size ? *cluster.map_shared_rank(&h.own[code_of(bin)], q + j) : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c += part[j];
+        }
+        for (int q = 0; q < r.size; ++q) *cluster.map_shared_rank(&h.all[bin], q) = c;
+    }
+    u64 own_tiny = 0;
+    if (TY == 0) {
+        const int tiny = int(h.own[2 * kCodes]);
+        own_tiny = block_reduce(r.sh, Pair{int(threadIdx.x) < tiny ? r.weight(h.tiny[threadIdx.x]) : 0, 0}, add_pairs).a;
+        if (int(threadIdx.x) < r.size) *cluster.map_shared_rank(&h.tiny_mass[r.rank], threadIdx.x) = own_tiny;
+    }
+    cluster.sync();
+    return own_tiny;
+}
+
+// A row whose counts are whole: every logit has a bin, or no weight.  Returns
+// false, in every CTA alike, where a cut of a bf16 row falls among its tiny
+// logits; such a row goes the general way.
+template <int TY>
+__device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, float u, float floor_v, bool greedy,
+                            Partition z) {
     Shared& sh = r.sh;
     Values& h = sh.values;
     auto cluster = cg::this_cluster();
-    const int tid = threadIdx.x, size = r.size;
-    const auto code_of = [](int bin) { return bin < kTinyBin ? kCodes - 1 - bin : bin == kTinyBin ? 2 * kCodes : bin - 1; };
-    const auto value_of = [](int bin) {
-        const int magnitude = bin < kTinyBin ? kCodes - 1 - bin : bin - 1 - kCodes;
-        const float v = __uint_as_float(uint32_t(magnitude + (115 << 7)) << 16);
-        return bin < kTinyBin ? v : bin == kTinyBin ? 0.f : -v;
-    };
-    const int per = (kValueBins + size - 1) / size;
-    for (int i = tid; i < per; i += kThreads) {
-        const int bin = r.rank * per + i;
-        if (bin >= kValueBins) break;
-        const int code = code_of(bin);
-        uint32_t c = 0;
-        for (int q = 0; q < size; ++q) c += *cluster.map_shared_rank(&h.own[code], q);
-        for (int q = 0; q < size; ++q) *cluster.map_shared_rank(&h.all[bin], q) = c;
-    }
-    auto add = [](Pair x, Pair y) { return Pair{x.a + y.a, x.b + y.b}; };
-    const u64 own_tiny =
-        block_reduce(sh, Pair{tid < int(h.own[2 * kCodes]) ? r.weight(h.tiny[tid]) : 0, 0}, add).a;
-    if (tid < size) *cluster.map_shared_rank(&h.tiny_mass[r.rank], tid) = own_tiny;
-    cluster.sync();
+    const int tid = threadIdx.x;
+    const u64 own_tiny = merge_counts(r);
+    const u64 limit = greedy ? 1 : k > 0 && k < a.vocab ? u64(k) : ~u64(0);
+    if (greedy) p = 1.f;
 
-    // this thread's values, largest first
+    // this thread's bins, largest values first; the border of top-k
     const int first = tid * kPerThread;
     uint32_t cnt[kPerThread];
-    u64 weight[kPerThread], count = 0, tiny_mass = 0;
-    for (int q = 0; q < size; ++q) tiny_mass += h.tiny_mass[q];
+    u64 count = 0;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-        const float v = value_of(first + i);
-        cnt[i] = v >= floor_v ? h.all[first + i] : 0;
-        weight[i] = cnt[i] ? (greedy ? 1 : r.weight(v)) : 0;
+        cnt[i] = (TY == 0 ? near_edge(first + i) : bin_top(first + i)) >= floor_v ? h.all[first + i] : 0;
         count += cnt[i];
     }
     if (tid == 0) sh.found = 0;
-    const bool by_count = greedy || (k > 0 && k < a.vocab);
-    const u64 limit = greedy ? 1 : u64(k);
-    u64 mass = 0;
-    const u64 before = by_count ? block_exclusive(sh, count) : 0;
-    u64 seen = before;
+    u64 seen = block_exclusive(sh, count);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-        const int bin = first + i;
+        if (seen < limit && limit <= seen + cnt[i])
+            sh.found = 1, sh.found_bin = first + i, sh.bound[0] = seen, sh.bound[1] = seen + cnt[i];
         const uint32_t had = cnt[i];
-        if (by_count) {
-            cnt[i] = seen >= limit ? 0 : uint32_t(min(u64(had), limit - seen));
-            if (seen < limit && limit <= seen + had) {
-                sh.found = 1, sh.found_bin = bin, sh.bound[1] = limit - seen;
-                if (bin == kTinyBin && cnt[i] < had) sh.found = 2;
-            }
-            seen += had;
-        }
-        mass += bin == kTinyBin ? (cnt[i] ? tiny_mass : 0) : cnt[i] * weight[i];
-    }
-    if (p < 1.f && !greedy) {
-        const u64 ahead = block_exclusive(sh, mass);
-        if (tid == kThreads - 1) sh.bound[0] = ahead + mass;
-        __syncthreads();
-        const u64 total = sh.bound[0];
-        const bool stuck = sh.found == 2;
-        __syncthreads();  // found and bound are written again below
-        if (stuck) return false;
-        const u64 share = __double2ull_rz(double(p) * 0x1p64);
-        const u64 target = max(u64(1), __umul64hi(total, share) + (total * share != 0));
-        if (ahead < target && target <= ahead + mass) {
-            u64 at = ahead;
-#pragma unroll
-            for (int i = 0; i < kPerThread; ++i) {
-                const int bin = first + i;
-                const u64 m = bin == kTinyBin ? (cnt[i] ? tiny_mass : 0) : cnt[i] * weight[i];
-                if (at < target && target <= at + m) {
-                    sh.found = 1, sh.found_bin = bin;
-                    if (bin == kTinyBin)
-                        sh.found = 2;
-                    else
-                        sh.bound[1] = (target - at + weight[i] - 1) / weight[i];
-                }
-                at += m;
-            }
-        }
+        cnt[i] = seen >= limit ? 0 : uint32_t(min(u64(had), limit - seen));
+        seen += had;
     }
     __syncthreads();
-    if (sh.found == 2) return false;
-    const int border = sh.found ? sh.found_bin : INT_MAX;
-    const u64 ties = sh.bound[1];  // kept of the border's value
-    u64 here = 0, mine = 0;        // of that value in this CTA, and of the kept
-    if (sh.found) {
-        // counts of the border's value in the CTAs before this one
-        if (tid < size) sh.slab[tid] = *cluster.map_shared_rank(&h.own[code_of(border)], tid);
-        __syncthreads();
-        u64 prior = 0;
-        for (int q = 0; q < r.rank; ++q) prior += sh.slab[q];
-        here = sh.slab[r.rank];
-        mine = prior >= ties ? 0 : min(here, ties - prior);
-    }
-    mass = 0;
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-        const int bin = first + i;
-        if (bin == border)
-            mass += mine * (bin == kTinyBin ? 0 : weight[i]);
-        else if (bin < border && bin < kValueBins && bin != kTinyBin && weight[i])
-            mass += h.own[code_of(bin)] * weight[i];
-    }
-    if (tid == 0 && border >= kTinyBin && floor_v <= 0.f) mass += own_tiny;
-    const Pair own = block_reduce(sh, Pair{mass, 0}, add);
-    const Pair* box = r.exchange(own);
-    u64 whole = 0, ahead = 0;
-    for (int q = 0; q < size; ++q) {
-        if (q < r.rank) ahead += box[q].a;
-        whole += box[q].a;
-    }
-    const u64 target = __umul64hi(whole, __double2ull_rz(double(u) * 0x1p64));  // floor(u * mass): token has sum > it
-    if (ahead > target || target >= ahead + own.a) return true;
-
-    // The CTA that holds the token.
-    r.cut_v = floor_v, r.cut_i = INT_MAX;
-    if (floor_v == -INFINITY) r.cut_i = -1;
-    if (border != INT_MAX) {
-        r.cut_v = value_of(border);
-        if (border == kTinyBin)
-            r.cut_v = -0x1p-12f, r.cut_i = -1;  // all of the tiny
-        else if (mine == here)
-            r.cut_i = INT_MAX;
-        else
-            r.cut_i = mine ? nth_equal(r, r.cut_v, mine) : -1;
-    }
-    Partition z{1.0, 0.0};
-    if (a.logprobs) {
-        float others = 0.f, tops = 0.f;
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            const float v = value_of(first + i), c = float(h.all[first + i]);
-            if (v == r.top)
-                tops += c;
-            else if (c > 0.f)
-                others = __fmaf_rn(c, expf(__fsub_rn(v, r.top)), others);
-        }
-        const Pair sums = block_reduce(
-            sh, Pair{u64(__double_as_longlong(tops)), u64(__double_as_longlong(others))}, add_doubles);
-        z.tops = __longlong_as_double(sums.a), z.others = __longlong_as_double(sums.b);
-    }
-    const int turns = (a.vecs + kThreads - 1) / kThreads;
-    if (greedy) {
-        // the border is the largest logit and the token its first
-        const int index = nth_equal(r, r.top, 1);
-        if (tid == 0) {
-            a.tokens[row] = index;
-            if (a.logprobs) a.logprobs[row] = z.of(r.top, r.top);
+    const bool by_count = sh.found;
+    int border = by_count ? sh.found_bin : INT_MAX;
+    const u64 before = sh.bound[0], listed = sh.bound[1];
+    if (by_count && listed <= u64(kCap)) {
+        push_list(r, fmaxf(TY == 0 && border != kTinyBin ? near_edge(border) : bin_bottom(border), floor_v));
+        cluster.sync();
+        if (r.rank == 0) {
+            if constexpr (TY == 0)
+                if (a.logprobs) z = partition_of(r);
+            draw_from_list(r, a, row, limit, p, u, 0, z);
         }
         return true;
     }
-    slab_masses(r, turns);
-    __syncthreads();
-    if (tid < 32) write_token(r, a, row, ahead, target, turns, z);
-    return true;
+
+    if constexpr (TY == 0) {
+        u64 ties = by_count ? limit - before : 0;  // kept of the border's value
+        if (by_count && border == kTinyBin && limit < listed) return false;
+        u64 tiny_mass = 0;
+        for (int q = 0; q < r.size; ++q) tiny_mass += h.tiny_mass[q];
+        u64 weight[kPerThread], mass = 0;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            weight[i] = cnt[i] ? r.weight(near_edge(first + i)) : 0;
+            mass += first + i == kTinyBin ? (cnt[i] ? tiny_mass : 0) : cnt[i] * weight[i];
+        }
+        if (p < 1.f) {
+            const u64 ahead = block_exclusive(sh, mass);
+            if (tid == kThreads - 1) sh.bound[0] = ahead + mass;
+            __syncthreads();
+            const u64 whole = sh.bound[0], target = nucleus(whole, p);
+            if (ahead < target && target <= ahead + mass) {
+                u64 at = ahead, w = 0, kept = 0;
+                int bin = 0;
+                u64 c = seen - count;  // tokens above this thread's bins
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) {
+                    const u64 m = first + i == kTinyBin ? (cnt[i] ? tiny_mass : 0) : cnt[i] * weight[i];
+                    c += cnt[i];
+                    if (at < target && target <= at + m) bin = first + i, w = weight[i], sh.bound[1] = at, kept = c;
+                    at += m;
+                }
+                sh.found_bin = bin, sh.found = int(min(kept, u64(INT_MAX)));
+                if (bin != kTinyBin) sh.bound[1] = ceil_div(target - sh.bound[1], w);
+            }
+            __syncthreads();
+            border = sh.found_bin, ties = sh.bound[1];
+            if (border == kTinyBin) return false;
+            if (sh.found <= kCap) {
+                push_list(r, near_edge(border));
+                cluster.sync();
+                if (r.rank == 0) {
+                    if (a.logprobs) z = partition_of(r);
+                    draw_from_list(r, a, row, limit, p, u, whole, z);
+                }
+                return true;
+            }
+        }
+        u64 here = 0, mine = 0;  // of the border's value in this CTA, and of the kept
+        if (border != INT_MAX) {
+            // counts of the border's value in the CTAs before this one
+            if (tid < r.size) sh.slab[tid] = *cluster.map_shared_rank(&h.own[code_of(border)], tid);
+            __syncthreads();
+            u64 prior = 0;
+            for (int q = 0; q < r.rank; ++q) prior += sh.slab[q];
+            here = sh.slab[r.rank];
+            mine = prior >= ties ? 0 : min(here, ties - prior);
+        }
+        mass = 0;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            const int bin = first + i;
+            if (bin != kTinyBin && weight[i] && bin <= border)
+                mass += (bin == border ? mine : h.own[code_of(bin)]) * weight[i];
+        }
+        if (tid == 0 && border >= kTinyBin && floor_v <= 0.f) mass += own_tiny;
+        const Pair own = block_reduce(sh, Pair{mass, 0}, add_pairs);
+        const Pair* all = r.exchange(own);
+        u64 whole = 0, ahead = 0;
+        for (int q = 0; q < r.size; ++q) {
+            if (q < r.rank) ahead += all[q].a;
+            whole += all[q].a;
+        }
+        const u64 target = drawn(whole, u);
+        if (ahead > target || target >= ahead + own.a) return true;
+        // the CTA that holds the token
+        if (a.logprobs) z = partition_of(r);
+        r.cut_v = floor_v, r.cut_i = floor_v == -INFINITY ? -1 : INT_MAX;
+        if (border == kTinyBin) {
+            r.cut_v = bin_bottom(kTinyBin), r.cut_i = INT_MAX;  // all of the tiny
+        } else if (border != INT_MAX) {
+            r.cut_v = near_edge(border), r.cut_i = mine ? INT_MAX : -1;
+            if (mine && mine < here) r.cut_i = nth_equal(r, r.cut_v, mine);
+        }
+        const int turns = (a.vecs + kThreads - 1) / kThreads;
+        slab_masses(r, turns);
+        __syncthreads();
+        if (tid < 32) write_token(r, a, row, ahead, target, turns, z);
+        return true;
+    } else {
+        r.cut_v = floor_v, r.cut_i = floor_v == -INFINITY ? -1 : INT_MAX;
+        // the search below uses the histogram's memory: the counts are in registers, and its own exchanges wait for all
+        if (p < 1.f) {
+            // Bounds of the bins' masses, and with them of the nucleus' border: it lies in the bins from the
+            // first that can reach it to the first that must.
+            double low = 0.0, high = 0.0;
+            double lower[kPerThread], upper[kPerThread];
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                lower[i] = upper[i] = 0.0;
+                if (cnt[i]) {
+                    const float bottom = bin_bottom(first + i), above = bin_top(first + i);
+                    upper[i] = double(cnt[i]) * double(r.weight(fminf(above, r.top)) + 1);
+                    if (bottom >= floor_v) lower[i] = double(cnt[i]) * double(r.weight(bottom));
+                }
+                low += lower[i], high += upper[i];
+            }
+            const Pair ends{u64(__double_as_longlong(low)), u64(__double_as_longlong(high))};
+            const auto add = [](Pair x, Pair y) {
+                return Pair{u64(__double_as_longlong(__longlong_as_double(x.a) + __longlong_as_double(y.a))),
+                            u64(__double_as_longlong(__longlong_as_double(x.b) + __longlong_as_double(y.b)))};
+            };
+            const Pair total = block_reduce(sh, ends, add);
+            const double can = double(p) * __longlong_as_double(total.a) * (1.0 - 1e-9);
+            const double must = double(p) * __longlong_as_double(total.b) * (1.0 + 1e-9);
+            // sums in another order differ in the last bits: the margins above are far wider
+            double at_low = block_exclusive_double(sh, low), at_high = block_exclusive_double(sh, high);
+            if (tid == 0) sh.found_bin = 0, sh.found = kValueBins - 1, sh.bound[0] = 0;
+            __syncthreads();
+            u64 c = seen - count;
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                if (at_high < can && can <= at_high + upper[i]) sh.found_bin = first + i;
+                if (at_low < must && must <= at_low + lower[i]) sh.found = first + i;
+                at_high += upper[i], at_low += lower[i], c += cnt[i];
+            }
+            __syncthreads();
+            const int open = sh.found_bin, close = sh.found;
+            // tokens above the first bin and up to the last
+            const u64 counts_open = count_above(sh, first, seen - count, cnt, open);
+            const u64 counts_close = count_above(sh, first, seen - count, cnt, close + 1);
+            if (by_count) cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
+            const float edge = bin_top(open);
+            const bool few = counts_close <= u64(kCap) && !by_count;
+            if (few) push_list(r, fmaxf(bin_bottom(close), floor_v));
+            u64 mass = 0, above = 0;
+            r.each([&](float x, int slot) {
+                if (r.kept(x, slot)) {
+                    const u64 w = r.weight(x);
+                    mass += w;
+                    if (x > edge) above += w;
+                }
+            });
+            const Pair* all = r.exchange(block_reduce(sh, Pair{mass, above}, add_pairs));
+            Pair sums{0, 0};
+            for (int q = 0; q < r.size; ++q) sums = add_pairs(sums, all[q]);
+            if (few) {
+                if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, sums.a, z);
+                return true;
+            }
+            cut_row<TY, true>(r, fmaxf(bin_bottom(close), floor_v), edge, sums.b, nucleus(sums.a, p), counts_close - counts_open);
+        } else if (by_count) {
+            cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
+        }
+        draw_from_row(r, a, row, u, z);
+        return true;
+    }
 }
 
 // The values of a 16-byte vector of which only a part lies in the row.
@@ -705,29 +936,15 @@ __device__ __forceinline__ uint4 edge_vector(const char* begin, int i0, int voca
 // CTAs are resident together and take every barrier, as all decisions that
 // lead to one are taken from exchanged values.
 template <int TY>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     using El = Elem<TY>;
     constexpr int E = El::E, kBatch = 4;
     extern __shared__ uint4 data[];
     __shared__ Shared sh;
     auto cluster = cg::this_cluster();
+    cluster.barrier_arrive();  // waited for before the first access to another CTA's shared memory
     const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
     const int row = blockIdx.x / size, tid = threadIdx.x;
-
-    const float T = a.temperature ? a.temperature[row] : 1.f;
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, u = a.uniform[row];
-    if (!(T >= 0.f && T <= kMaxTemperature) || !(p >= 0.f) || !(min_p >= 0.f && min_p <= 1.f) ||
-        !(u >= 0.f && u < 1.f)) {
-        if (rank == 0 && tid == 0) {
-            a.tokens[row] = -1;
-            if (a.logprobs) a.logprobs[row] = NAN;
-            atomicOr(a.flags, kFlagParameter);
-        }
-        return;
-    }
-    cluster.barrier_arrive();  // waited for before the first access to another CTA's shared memory
-    const bool greedy = T == 0.f || k == 1;
 
     // this CTA's share of the row: whole 16-byte vectors of memory, values outside the row as -inf
     const char* begin = static_cast<const char*>(a.logits) + int64_t(row) * a.stride * El::kBytes;
@@ -736,25 +953,44 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
     const int v0 = min(rank * a.vecs, total_vecs), nvec = min(a.vecs, total_vecs - v0);
     const uint4* base = reinterpret_cast<const uint4*>(begin - lead * El::kBytes) + v0;
     const int i_first = v0 * E - lead;  // index of the first value
-    float top = -INFINITY;
-    uint32_t notes = 0;  // 1: NaN or +inf; bf16: 2: 128 or more, 4: -128 or less but not -inf, 8: too many tiny
-    for (int b = 0; b == 0 || b < nvec; b += kBatch * kThreads) {
-        uint4 q[kBatch];
+    uint4 q[kBatch];
+    auto fetch = [&](int b) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const int v = b + j * kThreads + tid, i0 = i_first + v * E;
             if (v < nvec)
                 q[j] = i0 >= 0 && i0 + E <= a.vocab ? __ldcs(base + v) : edge_vector<TY>(begin, i0, a.vocab);
         }
-        if (b == 0) {
-            if (tid < 64) sh.pow64[tid] = exp2(-tid * (1.0 / 64));
-            if (TY == 0) {
-                for (int i = tid; i < kValueBins; i += kThreads) sh.values.own[i] = 0;
-                for (int i = kValueBins + tid; i < kPerThread * kThreads; i += kThreads) sh.values.all[i] = 0;
-                if (tid == 0) sh.values.tiny_n = 0;
-                __syncthreads();
-            }
+    };
+    fetch(0);
+
+    const float T = a.temperature ? a.temperature[row] : 1.f;
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, u = a.uniform[row];
+    const bool valid = T >= 0.f && T <= kMaxTemperature && p >= 0.f && min_p >= 0.f && min_p <= 1.f && u >= 0.f && u < 1.f;
+    if (!valid) {
+        if (rank == 0 && tid == 0) {
+            a.tokens[row] = -1;
+            if (a.logprobs) a.logprobs[row] = NAN;
+            atomicOr(a.flags, kFlagParameter);
         }
+        cluster.barrier_wait();
+        return;
+    }
+    const bool greedy = T == 0.f || k == 1, cuts = greedy || (k > 0 && k < a.vocab) || p < 1.f;
+    const bool counting = TY == 0 || cuts;
+    Values& h = sh.values;
+    if (counting) {
+        for (int i = tid; i < kValueBins; i += kThreads) h.own[i] = 0;
+        for (int i = kValueBins + tid; i < kPerThread * kThreads; i += kThreads) h.all[i] = 0;
+    }
+    if (tid < 64) sh.pow64[tid] = exp2(-tid * (1.0 / 64));
+    if (tid == 0) sh.list.n = 0;
+    __syncthreads();
+    float top = -INFINITY;
+    uint32_t notes = 0;  // 1: NaN or +inf; 2: 128 or more, 4: -128 or less but not -inf, 8: too many tiny
+    for (int b = 0; b < nvec; b += kBatch * kThreads) {
+        if (b) fetch(b);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const int v = b + j * kThreads + tid;
@@ -765,15 +1001,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 top = fmaxf(top, x[e]);
-                if (TY == 0) {
+                if (counting) {
                     const uint32_t bits = __float_as_uint(x[e]) >> 16, magnitude = bits & 0x7fffu;
-                    const uint32_t code = magnitude - (115u << 7);
+                    const uint32_t code = magnitude - kFirstCode;
                     if (code < uint32_t(kCodes)) {
-                        atomicAdd(&sh.values.own[code + (bits >> 15) * kCodes], 1u);
-                    } else if (magnitude < (115u << 7)) {
-                        const uint32_t at = atomicAdd(&sh.values.tiny_n, 1u);
-                        if (at < uint32_t(kTinyCap)) sh.values.tiny[at] = x[e];
-                        else notes |= 8;
+                        atomicAdd(&h.own[code + (bits >> 15) * kCodes], 1u);
+                    } else if (magnitude < kFirstCode) {
+                        const uint32_t at = atomicAdd(&h.own[2 * kCodes], 1u);
+                        if (TY == 0) {
+                            if (at < uint32_t(kTinyCap)) h.tiny[at] = x[e];
+                            else notes |= 8;
+                        }
                     } else if (!(x[e] < INFINITY)) {
                         notes |= 1;
                     } else if (x[e] != -INFINITY) {
@@ -788,12 +1026,24 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
 
     Row<TY> r{sh, data, nvec, i_first, rank, size, 0};
     auto join = [](Pair x, Pair y) { return Pair{as_bits(fmaxf(as_float(x.a), as_float(y.a))), x.b | y.b}; };
-    Pair own = block_reduce(sh, Pair{as_bits(top), notes}, join);
-    if (TY == 0 && tid == 0) sh.values.own[2 * kCodes] = min(sh.values.tiny_n, uint32_t(kTinyCap));
+    const Pair mine = block_reduce(sh, Pair{as_bits(top), notes}, join);
+    // sum of exponentials for the log probability, against this CTA's largest logit; a bf16 row takes it from its counts
+    Pair sums{0, 0};
+    if (TY != 0 && a.logprobs) {
+        const float local = as_float(mine.a);
+        float equal = 0.f, others = 0.f;
+        r.each([&](float x, int) {
+            if (x == local)
+                equal += 1.f;
+            else
+                others += expf(__fsub_rn(x, local));
+        });
+        sums = block_reduce(sh, Pair{as_bits(equal), as_bits(others)}, add_floats);
+    }
     cluster.barrier_wait();
-    const Pair* all = r.exchange(own);
-    for (int q = 0; q < size; ++q) own = join(own, all[q]);
-    top = as_float(own.a), notes = uint32_t(own.b);
+    const Pair* all = r.exchange(Pair{mine.a | mine.b << 32, sums.a | sums.b << 32});
+    top = -INFINITY, notes = 0;
+    for (int i = 0; i < size; ++i) top = fmaxf(top, as_float(all[i].a)), notes |= uint32_t(all[i].a >> 32);
     if ((notes & 1) || top == -INFINITY) {
         if (rank == 0 && tid == 0) {
             a.tokens[row] = -1;
@@ -802,96 +1052,78 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
         }
         return;
     }
+    Partition z{0.f, 0.f};
+    if (TY != 0 && a.logprobs)
+        for (int i = 0; i < size; ++i) {
+            const float local = as_float(all[i].a), equal = as_float(all[i].b), others = as_float(all[i].b >> 32);
+            if (local == top)
+                z.tops += equal, z.others += others;
+            else if (local > -INFINITY)
+                z.others = __fmaf_rn(__fadd_rn(equal, others), expf(__fsub_rn(local, top)), z.others);
+        }
     r.top = top;
     r.step = greedy ? 0.0 : 64.0 * 1.4426950408889634074 / double(T);
     r.frac = min(51, 62 - (32 - __clz((a.vocab - 1) | 1)));
-    r.count_mode = false;
+    r.count_mode = u == 0.f && !greedy;
     // w >= min_p as a comparison of logits, which is exact
     float floor_v = -INFINITY;
     if (min_p > 0.f && !greedy) floor_v = __double2float_ru(double(top) + double(T) * log(double(min_p)));
-    if (TY == 0) {
-        // Every logit but the tiny ones has a code of its own, or no weight: below -128 that takes 37 T.
+    r.cut_v = floor_v, r.cut_i = floor_v == -INFINITY ? -1 : INT_MAX;
+    if (counting) {
+        // The counts must hold every logit that has a weight: below -128 none has from 37 T on.  A bf16 row also
+        // needs its largest logit and min-p's border outside the tiny bin, where values are not told apart.
         const float heat = greedy ? 1.f : fmaxf(T, 1.f);
-        if (!(notes & 10) && top > -128.f && fabsf(top) >= 0x1p-12f && u != 0.f &&
-            (!(notes & 4) || top + 128.f >= 37.f * heat) && !(fabsf(floor_v) < 0x1p-12f)) {
-            if constexpr (TY == 0)
-                if (value_row(r, a, row, T, k, p, u, floor_v, greedy)) return;
-        }
-        cluster.sync();  // the histogram's memory is used again
+        bool whole = !(notes & 10) && top > -128.f && !r.count_mode && (!(notes & 4) || top + 128.f >= 37.f * heat);
+        if (TY == 0) whole = whole && fabsf(top) > bin_top(kTinyBin) && !(fabsf(floor_v) <= bin_top(kTinyBin));
+        if (whole && counted_row(r, a, row, k, p, u, floor_v, greedy, z)) return;
+        cluster.sync();  // the counts' memory is used again
     }
 
-    // the smallest logit but -inf and the type's lowest value, which usually masks
-    float low = INFINITY;
-    r.each([&](float x, int) {
-        if (x > El::kLowest) low = fminf(low, x);
-    });
-    // log sum exp over all tokens: the largest logits counted, the others summed
-    Partition z{1.0, 0.0};
-    float others = 0.f, equal = 0.f;
-    if (a.logprobs)
+    // The general way: rows without a cut, and those that the counts do not tell enough about.
+    if (TY == 0 && a.logprobs) {
+        float equal = 0.f, others = 0.f;
         r.each([&](float x, int) {
             if (x == top)
                 equal += 1.f;
             else
                 others += expf(__fsub_rn(x, top));
         });
-    auto least = [](Pair x, Pair y) { return Pair{as_bits(fminf(as_float(x.a), as_float(y.a))), 0}; };
-    own = block_reduce(sh, Pair{as_bits(low), 0}, least);
-    low = as_float(own.a);
-    if (a.logprobs) {
-        own = block_reduce(sh, Pair{u64(__double_as_longlong(equal)), u64(__double_as_longlong(others))}, add_doubles);
+        const Pair own = block_reduce(sh, Pair{as_bits(equal), as_bits(others)}, add_floats);
         all = r.exchange(own);
-        own = all[0];
-        for (int q = 1; q < size; ++q) own = add_doubles(own, all[q]);
-        z.tops = __longlong_as_double(own.a), z.others = __longlong_as_double(own.b);
+        for (int i = 0; i < size; ++i) z.tops += as_float(all[i].a), z.others += as_float(all[i].b);
     }
-
-    if (greedy) {
-        int index = INT_MAX;
-        r.each([&](float x, int slot) {
-            if (x == top) index = min(index, r.first + slot);
+    const bool by_count = greedy || (k > 0 && k < a.vocab), by_mass = p < 1.f && !greedy;
+    if (by_count || by_mass) {
+        // The values that a cut searches: from the smallest logit but -inf and the type's lowest value, which usually
+        // masks.  Below 746 T under the top every weight is zero in double precision, so the order there never
+        // matters; in fixed point that holds from 37 T (2^-53) on.
+        float low = INFINITY;
+        r.each([&](float x, int) {
+            if (x > El::kLowest) low = fminf(low, x);
         });
-        auto first = [](Pair x, Pair y) { return Pair{min(x.a, y.a), 0}; };
-        own = block_reduce(sh, Pair{u64(index), 0}, first);
-        all = r.exchange(own);
-        for (int q = 0; q < size; ++q) own = first(own, all[q]);
-        if (rank == 0 && tid == 0) {
-            a.tokens[row] = int(own.a);
-            if (a.logprobs) a.logprobs[row] = z.of(top, top);
-        }
-        return;
-    }
-
-    r.cut_v = floor_v, r.cut_i = min_p > 0.f ? INT_MAX : -1;
-    if ((k > 0 && k < a.vocab) || p < 1.f) {
-        all = r.exchange(Pair{as_bits(low), 0});
-        for (int q = 0; q < size; ++q) low = fminf(low, as_float(all[q].a));
-        // The values a cut searches.  Below 746 T under the top every weight is
-        // zero in double precision, so the order there never matters; in fixed
-        // point that holds from 37 T (2^-53) on.
+        auto least = [](Pair x, Pair y) { return Pair{as_bits(fminf(as_float(x.a), as_float(y.a))), 0}; };
+        all = r.exchange(block_reduce(sh, Pair{as_bits(low), 0}, least));
+        for (int i = 0; i < size; ++i) low = fminf(low, as_float(all[i].a));
         if (double(top) - 746.0 * double(T) <= double(El::kLowest)) low = El::kLowest;
+        const auto from = [&](double units) {
+            return fminf(top, fmaxf(fmaxf(low, __double2float_rd(double(top) - units * double(T))), floor_v));
+        };
+        if (by_count) cut_row<TY, false>(r, from(746.0), top, 0, greedy ? 1 : u64(k), a.vocab);
+        if (by_mass) {
+            const bool counted = r.count_mode;
+            r.count_mode = false;  // the nucleus goes by mass for u = 0 too
+            u64 mass = 0;
+            r.each([&](float x, int slot) {
+                if (r.kept(x, slot)) mass += r.weight(x);
+            });
+            all = r.exchange(block_reduce(sh, Pair{mass, 0}, add_pairs));
+            mass = 0;
+            for (int i = 0; i < size; ++i) mass += all[i].a;
+            cut_row<TY, true>(r, from(37.0), top, 0, nucleus(mass, p), a.vocab);
+            r.count_mode = counted;
+        }
     }
-    if (k > 0 && k < a.vocab) {
-        const float floor_k = fmaxf(low, __double2float_rd(double(top) - 746.0 * double(T)));
-        cut_row<TY, false>(r, fminf(top, fmaxf(floor_k, r.cut_v)), u64(k), 0);
-    }
-    if (p < 1.f) {
-        const float floor_p = fmaxf(low, __double2float_rd(double(top) - 37.0 * double(T)));
-        cut_row<TY, true>(r, fminf(top, fmaxf(floor_p, r.cut_v)), 0, __double2ull_rz(double(p) * 0x1p64));
-    }
-
-    r.count_mode = u == 0.f;
-    const int turns = (a.vecs + kThreads - 1) / kThreads;
-    auto add = [](Pair x, Pair y) { return Pair{x.a + y.a, 0}; };
-    own = block_reduce(sh, Pair{slab_masses(r, turns), 0}, add);
-    all = r.exchange(own);
-    u64 whole = 0, ahead = 0;
-    for (int q = 0; q < size; ++q) {
-        if (q < rank) ahead += all[q].a;
-        whole += all[q].a;
-    }
-    const u64 target = __umul64hi(whole, __double2ull_rz(double(u) * 0x1p64));  // floor(u * mass): token has sum > it
-    if (ahead <= target && target < ahead + own.a && tid < 32) write_token(r, a, row, ahead, target, turns, z);
+    draw_from_row(r, a, row, u, z);
 }
 
 std::atomic<bool> g_attr[3][64];
