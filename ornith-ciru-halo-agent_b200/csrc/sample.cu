@@ -13,11 +13,11 @@
 // the border between two tokens, where fp32 sums would choose another token
 // than the definition once in a few thousand draws.  Weights are therefore
 // 64-bit fixed point, w * 2^s with s = min(51, 62 - ceil(log2 V)): each is
-// computed in double precision (relative error below 1e-13) and rounded once;
+// computed in double precision (relative error below 2e-13) and rounded once;
 // sums of integers are exact and do not depend on their order, so the same
 // inputs give the same token whatever the launch shape.  The exponential is
-// table driven (Tang, 1989): 2^-n/64 from a table of 64 values times a Taylor
-// polynomial of degree 4 in the remainder.
+// table driven (Tang, 1989): 2^-n/256 from a table of 256 values times a Taylor
+// polynomial of degree 3 in the remainder (at most ln 2 / 512, so 2e-13 off).
 //
 // Layout of the work.  A cluster of 1 to 16 CTAs takes one row: every CTA
 // keeps its share of the logits in shared memory, so the row is read from HBM
@@ -53,8 +53,9 @@ using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kMaxVocab = 1 << 19, kSms = 148;
 constexpr int kBins = 1024, kCap = 256;
-constexpr int kMaxVecs = (kMaxVocab / 4 + 1 + kMaxCluster - 1) / kMaxCluster;       // 16-byte vectors of a CTA
-constexpr int kSlabs = (kMaxVecs + kThreads - 1) / kThreads * kWarps;               // (turn, warp) pairs of a CTA
+constexpr int kMaxVecs = 1 << 15, kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
+// 16-byte vectors of a CTA: at most, and kept on chip by one or two CTAs of an SM
+constexpr int kSlabs = kMaxVecs / 32;                        // (turn, warp) pairs of a CTA
 constexpr float kMaxTemperature = 1e30f;
 constexpr uint32_t kFlagNonfinite = 1, kFlagParameter = 2, kFlagNothingLeft = 4;
 
@@ -66,7 +67,8 @@ struct Args {
     int32_t* tokens;
     float* logprobs;
     uint32_t* flags;
-    int vocab, vecs;  // vecs: 16-byte vectors of the row that one CTA keeps
+    int vocab, vecs;  // vecs: 16-byte vectors of a row for one CTA
+    int resident;     // they stay in shared memory
 };
 
 template <int TY>
@@ -131,35 +133,36 @@ struct Search {
 // and all below 2^-10 as one.
 constexpr int kOctaves = 17, kCodes = kOctaves * 128;
 constexpr uint32_t kFirstCode = (134 - kOctaves) << 7;         // of 2^-10
-constexpr int kTinyBin = kCodes, kValueBins = 2 * kCodes + 1;  // by value, largest first; the tiny between
+// Bins by value, largest first: the tiny between, the negative from a multiple of 4 on (three bins stay empty).
+constexpr int kTinyBin = kCodes, kNegative = kCodes + 4, kValueBins = kNegative + kCodes;
 constexpr int kPerThread = (kValueBins + kThreads - 1) / kThreads, kTinyCap = 256;
 struct Values {
-    uint32_t own[kValueBins];                      // by code: positive, negative, tiny
-    uint32_t all[kPerThread * kThreads];           // the row's, by value
+    alignas(16) uint32_t own[2 * kCodes + 4];      // by code: positive, negative, tiny
+    alignas(16) uint32_t all[kPerThread * kThreads];  // the row's, by value
     float tiny[kTinyCap];                          // this CTA's tiny logits (bf16 rows)
     u64 tiny_mass[kMaxCluster];                    // pushed
 };
 
 // A bin's largest and smallest value; the same for bf16 but in the tiny one.
 __device__ __forceinline__ int code_of(int bin) {
-    return bin < kTinyBin ? kCodes - 1 - bin : bin == kTinyBin ? 2 * kCodes : bin - 1;
+    return bin < kTinyBin ? kCodes - 1 - bin : bin < kNegative ? 2 * kCodes : bin - kNegative + kCodes;
 }
 __device__ __forceinline__ uint32_t magnitude_of(int bin) {
-    return (uint32_t(bin < kTinyBin ? kCodes - 1 - bin : bin - 1 - kCodes) + kFirstCode) << 16;
+    return (uint32_t(bin < kTinyBin ? kCodes - 1 - bin : bin - kNegative) + kFirstCode) << 16;
 }
 __device__ __forceinline__ float near_edge(int bin) {  // the edge next to zero
-    if (bin == kTinyBin) return 0.f;
+    if (bin >= kTinyBin && bin < kNegative) return 0.f;
     return __uint_as_float(magnitude_of(bin) | (bin < kTinyBin ? 0u : 0x80000000u));
 }
 __device__ __forceinline__ float far_edge(int bin) {
     return __uint_as_float(__float_as_uint(near_edge(bin)) | 0xffffu);
 }
 __device__ __forceinline__ float bin_top(int bin) {
-    if (bin == kTinyBin) return __uint_as_float((kFirstCode << 16) - 1);
+    if (bin >= kTinyBin && bin < kNegative) return __uint_as_float((kFirstCode << 16) - 1);
     return bin < kTinyBin ? far_edge(bin) : near_edge(bin);
 }
 __device__ __forceinline__ float bin_bottom(int bin) {
-    if (bin == kTinyBin) return -__uint_as_float((kFirstCode << 16) - 1);
+    if (bin >= kTinyBin && bin < kNegative) return -__uint_as_float((kFirstCode << 16) - 1);
     return bin < kTinyBin ? near_edge(bin) : far_edge(bin);
 }
 
@@ -171,16 +174,17 @@ struct List {
     uint32_t n;
 };
 
-struct Shared {
+struct alignas(16) Shared {
     union {
         Search search;
         Values values;
     };
     List list;
-    double pow64[64];                    // 2^(-j/64)
+    double pow256[256];                  // 2^(s - j/256)
     Pair slot[2][kMaxCluster];           // pushed by every CTA of the cluster in turn
     u64 slab[kSlabs];                    // kept mass of each (turn, warp) in index order
     Pair red[kWarps];
+    Pair part[kMaxCluster];              // fp16, fp32: every CTA's largest logit, count of it and sum of the others
     u64 bound[2];
     int found, found_bin;
 };
@@ -188,50 +192,131 @@ struct Shared {
 __device__ __forceinline__ float as_float(u64 v) { return __uint_as_float(uint32_t(v)); }
 __device__ __forceinline__ u64 as_bits(float v) { return __float_as_uint(v); }
 
+// The values of a 16-byte vector of which only a part lies in the row.
+template <int TY>
+__device__ __forceinline__ uint4 edge_vector(const char* begin, int i0, int vocab) {
+    constexpr int E = Elem<TY>::E, kBytes = Elem<TY>::kBytes;
+    uint32_t w[4] = {Elem<TY>::kNone, Elem<TY>::kNone, Elem<TY>::kNone, Elem<TY>::kNone};
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (i0 + e >= 0 && i0 + e < vocab) {
+            if (kBytes == 2) {
+                const uint32_t h = reinterpret_cast<const uint16_t*>(begin)[i0 + e];
+                w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | h << 16 : (w[e / 2] & 0xffff0000u) | h;
+            } else {
+                w[e & 3] = reinterpret_cast<const uint32_t*>(begin)[i0 + e];
+            }
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // What every thread of a row's cluster knows.
 template <int TY>
 struct Row {
     using El = Elem<TY>;
+    static constexpr int E = El::E;
     Shared& sh;
-    const uint4* data;  // this CTA's vectors
-    int nvec, first;    // first: index of slot 0 (below 0 where the row starts inside a vector)
+    const uint4* data;    // this CTA's vectors in shared memory, or null
+    const uint4* source;  // and where they lie in the tensor
+    const char* begin;    // the row's first logit
+    int vocab, nvec, first;  // first: index of slot 0 (below 0 where the row starts inside a vector)
     int rank, size, parity;
-    float top;          // the largest logit
-    double step;        // 64 log2(e) / T
-    int frac;           // s of the fixed point
-    bool count_mode;    // u = 0: any token of positive weight counts as one
-    float cut_v;        // kept: x > cut_v, or x == cut_v and index <= cut_i
-    int cut_i;
+    float top;            // the largest logit
+    double step;          // 256 log2(e) / T
+    bool count_mode;      // u = 0: any token of positive weight counts as one
+    float weigh_from;     // no logit below this has a weight
+    float edge, tie_v;    // kept: x >= edge, or x == tie_v and index <= tie_i
+    int tie_i;
 
-    __device__ __forceinline__ bool kept(float x, int slot) const {
-        return x > cut_v || (x == cut_v && first + slot <= cut_i);
+    __device__ __forceinline__ uint4 vec(int v) const {
+        if (data) return data[v];
+        const int i0 = first + v * E;
+        return i0 >= 0 && i0 + E <= vocab ? __ldcg(source + v) : edge_vector<TY>(begin, i0, vocab);
     }
+    __device__ __forceinline__ bool kept(float x, int slot) const {
+        return x >= edge || (x == tie_v && first + slot <= tie_i);
+    }
+    __device__ void keep_from(float v) { edge = fmaxf(v, -FLT_MAX), tie_v = 0.f, tie_i = -1; }
+    __device__ void cut_at(float v, int index) { edge = nextafterf(v, INFINITY), tie_v = v, tie_i = index; }
 
     template <class F>
     __device__ __forceinline__ void each(F f) const {
+        if (int(threadIdx.x) >= nvec) return;
+        uint4 next = vec(threadIdx.x);
         for (int v = threadIdx.x; v < nvec; v += kThreads) {
-            float x[El::E];
-            El::unpack(data[v], x);
+            float x[E];
+            El::unpack(next, x);
+            if (v + kThreads < nvec) next = vec(v + kThreads);  // in flight meanwhile
 #pragma unroll
-            for (int e = 0; e < El::E; ++e) f(x[e], v * El::E + e);
+            for (int e = 0; e < E; ++e) f(x[e], v * E + e);
         }
     }
 
-    __device__ __forceinline__ u64 weight(float x) const {
-        const double y = __dmul_rn(__dsub_rn(double(top), double(x)), step);
-        if (count_mode) return y < 64.0 * 1074.0 ? 1 : 0;
-        if (!(y < 64.0 * (frac + 1))) return 0;  // below half a unit (and -inf)
-        const double shifted = __dadd_rn(y, 0x1.8p52);
+    // By mass, or (count) by number of tokens that have a weight in double precision.
+    __device__ void weigh(bool count, int frac, float T) {
+        count_mode = count;
+        weigh_from = fmaxf(-FLT_MAX, __double2float_ru(double(top) - (count ? 744.0 : 0.6931471805599453 * (frac + 1)) * double(T)));
+    }
+
+    // 2^52 + the fixed-point weight, as the bits of a double; 2^52 where not `in`.
+    __device__ __forceinline__ u64 raw_weight(float x, bool in) const {
+        constexpr double a = 0.69314718055994530942 / 256, kRound = 0x1.8p52;
+        const double d = __dsub_rn(double(top), double(x));
+        const double shifted = __fma_rn(d, step, kRound);  // n = rint(256 d log2(e) / T) in its low bits
         const int n = __double2loint(shifted);
-        const double f = __dsub_rn(y, __dsub_rn(shifted, 0x1.8p52));
-        constexpr double a = 0.69314718055994530942 / 64;
-        double p = __fma_rn(f, a * a * a * a / 24, -a * a * a / 6);
-        p = __fma_rn(p, f, a * a / 2);
+        const double f = __fma_rn(d, step, -__dsub_rn(shifted, kRound));
+        double p = __fma_rn(f, -a * a * a / 6, a * a / 2);
         p = __fma_rn(p, f, -a);
         p = __fma_rn(p, f, 1.0);
-        const double v = __dmul_rn(sh.pow64[n & 63], p);
-        const double scaled = __hiloint2double(__double2hiint(v) + ((frac - (n >> 6)) << 20), __double2loint(v));
-        return u64(__double_as_longlong(__dadd_rn(scaled, 0x1p52))) & 0xfffffffffffffull;
+        const double v = __dmul_rn(sh.pow256[n & 255], p);
+        const int high = __double2hiint(v) - ((n & ~255) << 12);  // times 2^-(n / 256)
+        return u64(__double_as_longlong(__dadd_rn(__hiloint2double(in ? high : 0, __double2loint(v)), 0x1p52)));
+    }
+    static constexpr u64 kRawZero = 0x4330000000000000ull;
+    __device__ __forceinline__ u64 weight(float x) const {
+        if (count_mode) return x >= weigh_from;
+        return raw_weight(x, x >= weigh_from) - kRawZero;
+    }
+    // Weights and their sum, without branches between them: a chain of double-precision steps is long, and its
+    // latency is hidden only by others beside it.
+    template <int N>
+    __device__ __forceinline__ void weights(const float (&x)[N], u64 (&w)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = raw_weight(x[i], x[i] >= weigh_from) - kRawZero;
+        if (count_mode) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = x[i] >= weigh_from;
+        }
+    }
+    // The kept mass of vector v, whose values are in q, and, at `above` or higher, a part of it.
+    template <bool PART>
+    __device__ __forceinline__ u64 kept_sum(int v, const uint4& q, float above, u64& part) const {
+        if (v >= nvec) return 0;
+        float x[E];
+        El::unpack(q, x);
+        bool in[E], any = false;
+        if (tie_i < 0) {  // no equal logits on both sides of the cut: one comparison each
+            const float from = fmaxf(edge, weigh_from);
+#pragma unroll
+            for (int e = 0; e < E; ++e) in[e] = x[e] >= from, any |= in[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) in[e] = kept(x[e], v * E + e) && x[e] >= weigh_from, any |= in[e];
+        }
+        if (!any) return 0;
+        u64 sum = 0;
+        if (count_mode) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum += in[e], part += PART && in[e] && x[e] >= above;
+            return sum;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const u64 raw = raw_weight(x[e], in[e]);
+            sum += raw;
+            if (PART) part += x[e] >= above ? raw - kRawZero : 0;
+        }
+        return sum - E * kRawZero;
     }
 
     // Everyone's pair, in rank order, after all have pushed theirs.  The two
@@ -287,23 +372,25 @@ __device__ __forceinline__ u64 block_exclusive(Shared& sh, u64 v) {
     return before + prior;
 }
 
-__device__ double block_exclusive_double(Shared& sh, double v) {
+// Exclusive prefixes of two floats per thread over the block.
+__device__ void block_exclusive_floats(Shared& sh, float a, float b, float& before_a, float& before_b) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double inc = v;
+    float ia = a, ib = b;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const double o = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += o;
+        const float oa = __shfl_up_sync(0xffffffffu, ia, d), ob = __shfl_up_sync(0xffffffffu, ib, d);
+        if (lane >= d) ia += oa, ib += ob;
     }
     __syncthreads();
-    if (lane == 31) sh.red[warp].a = u64(__double_as_longlong(inc));
+    if (lane == 31) sh.red[warp] = Pair{u64(__float_as_uint(ia)), u64(__float_as_uint(ib))};
     __syncthreads();
-    double before = 0.0;
+    before_a = __shfl_up_sync(0xffffffffu, ia, 1), before_b = __shfl_up_sync(0xffffffffu, ib, 1);
+    if (lane == 0) before_a = before_b = 0.f;
+    float wa = 0.f, wb = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
-        if (w < warp) before += __longlong_as_double(sh.red[w].a);
-    const double prior = __shfl_up_sync(0xffffffffu, inc, 1);
-    return lane ? before + prior : before;
+        if (w < warp) wa += __uint_as_float(uint32_t(sh.red[w].a)), wb += __uint_as_float(uint32_t(sh.red[w].b));
+    before_a += wa, before_b += wb;
 }
 
 // Tokens in the bins before `bin`, from counts that lie kPerThread to a thread.
@@ -328,26 +415,66 @@ __device__ __forceinline__ u64 ceil_div(u64 n, u64 d) {
     return q;
 }
 
+// Sums of slabs (turn, warp), in index order -> the slab that running sum
+// `target` falls into and the sum before it.  For one warp.
+__device__ __forceinline__ int find_slab(const Shared& sh, int slabs, u64 target, u64& sum) {
+    const int lane = threadIdx.x & 31, per_lane = (slabs + 31) / 32;
+    int slab = min(lane * per_lane, slabs);
+    const int end = min(slab + per_lane, slabs);
+    u64 part = 0;
+    for (int i = slab; i < end; ++i) part += sh.slab[i];
+    sum += warp_exclusive(part);
+    const bool here = sum <= target && target < sum + part;
+    if (here)
+        while (sum + sh.slab[slab] <= target) sum += sh.slab[slab++];
+    const int from = max(0, __ffs(__ballot_sync(0xffffffffu, here)) - 1);
+    slab = __shfl_sync(0xffffffffu, slab, from), sum = __shfl_sync(0xffffffffu, sum, from);
+    return slab;
+}
+__device__ __forceinline__ int slab_vector(int slab) {  // of a lane of the slab's warp
+    return (slab / kWarps) * kThreads + (slab % kWarps) * 32 + int(threadIdx.x & 31);
+}
+
 // The index of this CTA's `nth` kept token (from 1) whose logit is `value`; -1
 // where it has fewer.
 template <int TY>
 __device__ int nth_equal(const Row<TY>& r, float value, u64 nth) {
-    const int slots = r.nvec * Elem<TY>::E, per_thread = (slots + kThreads - 1) / kThreads;
-    const int s0 = min(int(threadIdx.x) * per_thread, slots), s1 = min(s0 + per_thread, slots);
-    const auto tie = [&](int slot) {
-        return Elem<TY>::one(reinterpret_cast<const char*>(r.data) + size_t(slot) * Elem<TY>::kBytes) == value &&
-               r.kept(value, slot);
+    constexpr int E = Elem<TY>::E;
+    Shared& sh = r.sh;
+    const int turns = (r.nvec + kThreads - 1) / kThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const auto ties = [&](int v, bool (&tie)[E]) {
+        float x[E];
+        if (v < r.nvec) Elem<TY>::unpack(r.vec(v), x);
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            tie[e] = v < r.nvec && x[e] == value && r.kept(x[e], v * E + e);
+            n += tie[e];
+        }
+        return n;
     };
-    u64 ties = 0;
-    for (int s = s0; s < s1; ++s) ties += tie(s);
-    u64 rankth = block_exclusive(r.sh, ties);
-    if (threadIdx.x == 0) r.sh.found_bin = -1;
+    __syncthreads();  // slab may still be read
+    if (threadIdx.x == 0) sh.found_bin = -1;
+    for (int turn = 0; turn < turns; ++turn) {
+        bool tie[E];
+        const uint32_t n = __reduce_add_sync(0xffffffffu, ties(turn * kThreads + int(threadIdx.x), tie));
+        if (lane == 0) sh.slab[turn * kWarps + warp] = n;
+    }
     __syncthreads();
-    if (rankth < nth && nth <= rankth + ties)
-        for (int s = s0; s < s1; ++s)
-            if (tie(s) && ++rankth == nth) r.sh.found_bin = r.first + s;
+    if (warp == 0 && nth > 0 && turns > 0) {
+        u64 sum = 0;
+        const int v = slab_vector(find_slab(sh, turns * kWarps, nth - 1, sum));
+        bool tie[E];
+        const uint32_t n = ties(v, tie);
+        u64 at = sum + warp_exclusive(n);
+        if (at < nth && nth <= at + n) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (tie[e] && ++at == nth) sh.found_bin = r.first + v * E + e;
+        }
+    }
     __syncthreads();
-    return r.sh.found_bin;
+    return sh.found_bin;
 }
 
 // Cuts the kept set inside [lo, hi], which holds at most `n` of it: `base`
@@ -398,7 +525,7 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
             all = r.exchange(Pair{u64(uint32_t(mine)), 0});
             int index = -1;
             for (int q = 0; q < r.size; ++q) index = max(index, int(uint32_t(all[q].a)));
-            if (index >= 0) r.cut_v = hi, r.cut_i = index;
+            if (index >= 0) r.cut_at(hi, index);
             return;
         }
         scale = __fdiv_rn(float(kBins), __fsub_rn(hi, lo));
@@ -484,7 +611,7 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
     const bool found = sh.found;
     if (mine && found && place == sh.found_bin) sh.bound[0] = as_bits(x), sh.bound[1] = u64(uint32_t(index));
     __syncthreads();
-    if (found) r.cut_v = as_float(sh.bound[0]), r.cut_i = int(uint32_t(sh.bound[1]));
+    if (found) r.cut_at(as_float(sh.bound[0]), int(uint32_t(sh.bound[1])));
     __syncthreads();
 }
 
@@ -492,30 +619,16 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
 // Vectors v = turn * kThreads + thread of a warp are consecutive in the row,
 // so slabs in order are in index order.
 template <int TY>
-__device__ __forceinline__ u64 vector_mass(const Row<TY>& r, int v, u64 (&w)[Elem<TY>::E]) {
-    constexpr int E = Elem<TY>::E;
-    u64 sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = 0;
-    if (v < r.nvec) {
-        float x[E];
-        Elem<TY>::unpack(r.data[v], x);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (r.kept(x[e], v * E + e)) w[e] = r.weight(x[e]);
-            sum += w[e];
-        }
-    }
-    return sum;
-}
-
-template <int TY>
-__device__ u64 slab_masses(const Row<TY>& r, int turns) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    u64 mine = 0;
+__device__ u64 slab_masses(const Row<TY>& r) {
+    const int turns = (r.nvec + kThreads - 1) / kThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 mine = 0, unused = 0;
+    __syncthreads();  // slab may still be read
+    uint4 next = int(threadIdx.x) < r.nvec ? r.vec(threadIdx.x) : uint4{};
     for (int turn = 0; turn < turns; ++turn) {
-        u64 w[Elem<TY>::E];
-        u64 sum = vector_mass(r, turn * kThreads + int(threadIdx.x), w);
+        const uint4 q = next;
+        const int v = turn * kThreads + int(threadIdx.x);
+        if (v + kThreads < r.nvec) next = r.vec(v + kThreads);  // in flight meanwhile
+        u64 sum = r.template kept_sum<false>(v, q, 0.f, unused);
         if (__any_sync(0xffffffffu, sum != 0)) {
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -524,6 +637,20 @@ __device__ u64 slab_masses(const Row<TY>& r, int turns) {
         mine += sum;
     }
     return lane == 0 ? mine : 0;
+}
+
+// The kept mass of this CTA, and that at `above` or higher, in this thread's vectors.
+template <int TY>
+__device__ Pair kept_mass(const Row<TY>& r, float above) {
+    Pair sum{0, 0};
+    uint4 next = int(threadIdx.x) < r.nvec ? r.vec(threadIdx.x) : uint4{};
+#pragma unroll 1
+    for (int v = threadIdx.x; v < r.nvec; v += kThreads) {
+        const uint4 q = next;
+        if (v + kThreads < r.nvec) next = r.vec(v + kThreads);  // in flight meanwhile
+        sum.a += r.template kept_sum<true>(v, q, above, sum.b);
+    }
+    return sum;
 }
 
 // The log probability of a token x: sums of exp(logit - top) over the largest
@@ -537,28 +664,21 @@ struct Partition {
 
 // One warp of the CTA that holds the token: its slab, its lane, its value.
 template <int TY>
-__device__ void write_token(const Row<TY>& r, const Args& a, int row, u64 ahead, u64 target, int turns,
-                            const Partition& z) {
+__device__ void write_token(const Row<TY>& r, const Args& a, int row, u64 ahead, u64 target, const Partition& z) {
     constexpr int E = Elem<TY>::E;
-    const Shared& sh = r.sh;
-    const int lane = threadIdx.x & 31;
-    const int slabs = turns * kWarps, per_lane = (slabs + 31) / 32;
-    int slab = lane * per_lane;
-    u64 part = 0;
-    for (int i = slab; i < min(slab + per_lane, slabs); ++i) part += sh.slab[i];
-    u64 sum = ahead + warp_exclusive(part);
-    const bool here = sum <= target && target < sum + part;
-    if (here)
-        while (sum + sh.slab[slab] <= target) sum += sh.slab[slab++];
-    const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-    slab = __shfl_sync(0xffffffffu, slab, from), sum = __shfl_sync(0xffffffffu, sum, from);
-    u64 w[E];
-    const int v = (slab / kWarps) * kThreads + (slab % kWarps) * 32 + lane;
-    const u64 vec = vector_mass(r, v, w);
-    u64 at = sum + warp_exclusive(vec);
+    const int turns = (r.nvec + kThreads - 1) / kThreads;
+    u64 at = ahead;
+    const int v = slab_vector(find_slab(r.sh, turns * kWarps, target, at));
+    float x[E];
+    u64 w[E], vec = 0;
+    if (v < r.nvec) Elem<TY>::unpack(r.vec(v), x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        w[e] = v < r.nvec && r.kept(x[e], v * E + e) ? r.weight(x[e]) : 0;
+        vec += w[e];
+    }
+    at += warp_exclusive(vec);
     if (at <= target && target < at + vec) {
-        float x[E];
-        Elem<TY>::unpack(r.data[v], x);
         bool done = false;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -585,8 +705,30 @@ __device__ __forceinline__ u64 nucleus(u64 mass, float p) {
     return max(u64(1), __umul64hi(mass, share) + (mass * share != 0));
 }
 
-// The largest logits and the others in a bf16 row's counts.
-__device__ Partition partition_of(Row<0>& r) {
+// The largest logits of a row and the others, from what every CTA has of them.
+// For a warp: every lane gets it.
+template <int TY>
+__device__ Partition joined_partition(const Row<TY>& r) {
+    Partition z{0.f, 0.f};
+    const int lane = threadIdx.x & 31;
+    if (lane < r.size) {
+        const Pair part = r.sh.part[lane];
+        const float local = as_float(part.a), equal = as_float(part.b), others = as_float(part.b >> 32);
+        if (local == r.top)
+            z = Partition{equal, others};
+        else if (local > -INFINITY)
+            z.others = __fmul_rn(__fadd_rn(equal, others), expf(__fsub_rn(local, r.top)));
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        z.tops += __shfl_xor_sync(0xffffffffu, z.tops, d);
+        z.others += __shfl_xor_sync(0xffffffffu, z.others, d);
+    }
+    return z;
+}
+
+// The same in a bf16 row's counts, for a block.
+__device__ Partition counted_partition(const Row<0>& r) {
     const Values& h = r.sh.values;
     float others = 0.f, tops = 0.f;
 #pragma unroll
@@ -594,11 +736,9 @@ __device__ Partition partition_of(Row<0>& r) {
         const int bin = int(threadIdx.x) * kPerThread + i;
         const float c = float(h.all[bin]);
         if (c > 0.f) {
-            const float v = near_edge(bin);
-            if (v == r.top)
-                tops = c;
-            else
-                others = __fmaf_rn(c, expf(__fsub_rn(v, r.top)), others);
+            const float v = near_edge(bin), e = expf(__fsub_rn(v, r.top));
+            tops = v == r.top ? c : tops;
+            others = v == r.top ? others : __fmaf_rn(c, e, others);
         }
     }
     const Pair sums = block_reduce(r.sh, Pair{as_bits(tops), as_bits(others)}, add_floats);
@@ -622,11 +762,17 @@ __device__ void push_list(const Row<TY>& r, float bottom) {
 // The first CTA ranks its list, applies top-k (`limit`) and top-p and draws.
 // `whole`: the mass that top-p refers to; 0: that of the first `limit`.
 template <int TY>
-__device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 limit, float p, float u, u64 whole,
-                               const Partition& z) {
+__device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 limit, float p, float u, u64 whole) {
     Shared& sh = r.sh;
     List& l = sh.list;
     const int tid = threadIdx.x, n = min(int(l.n), kCap);
+    Partition z{1.f, 0.f};
+    if (a.logprobs) {
+        if constexpr (TY == 0)
+            z = counted_partition(r);
+        else
+            z = joined_partition(r);
+    }
     // two threads a token; the order of the list varies, the ranks do not
     const int e = tid >> 1, half = tid & 1;
     int rank = 0;
@@ -669,9 +815,8 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
 
 // Kept masses of the CTAs -> the one that holds the token finds it.
 template <int TY>
-__device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, const Partition& z) {
-    const int turns = (a.vecs + kThreads - 1) / kThreads;
-    const Pair own = block_reduce(r.sh, Pair{slab_masses(r, turns), 0}, add_pairs);
+__device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u) {
+    const Pair own = block_reduce(r.sh, Pair{slab_masses(r), 0}, add_pairs);
     const Pair* all = r.exchange(own);
     u64 whole = 0, ahead = 0;
     for (int q = 0; q < r.size; ++q) {
@@ -679,34 +824,57 @@ __device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, const
         whole += all[q].a;
     }
     const u64 target = drawn(whole, u);
-    if (ahead <= target && target < ahead + own.a && threadIdx.x < 32) write_token(r, a, row, ahead, target, turns, z);
+    if (ahead <= target && target < ahead + own.a && threadIdx.x < 32)
+        write_token(r, a, row, ahead, target, a.logprobs ? joined_partition(r) : Partition{1.f, 0.f});
 }
 
 // The row's counts, by value, in every CTA; and for bf16 the mass of the tiny.
+// Each CTA adds up a range of codes, four at a time, in its own copy of the
+// result, and pushes that to the others.
 template <int TY>
-__device__ u64 merge_counts(const Row<TY>& r) {
+__device__ u64 merge_counts(const Row<TY>& r, uint32_t tiny_count) {
     Values& h = r.sh.values;
     auto cluster = cg::this_cluster();
-    const int per = (kValueBins + r.size - 1) / r.size;
-    for (int i = threadIdx.x; i < per; i += kThreads) {
-        const int bin = r.rank * per + i;
-        if (bin >= kValueBins) break;
-        uint32_t c = 0;
-        for (int q = 0; q < r.size; q += 8) {  // eight loads from other CTAs at a time
-            uint32_t part[8];
+    const int tid = threadIdx.x, quads = 2 * kCodes / 4 / r.size, first = r.rank * quads;
+    const auto place = [](int quad) {  // the bins of codes 4 * quad + {0..3}: backwards for the positive ones
+        return 4 * quad < kCodes ? kCodes - 4 - 4 * quad : kNegative + 4 * quad - kCodes;
+    };
+    const int teams = max(1, kThreads / quads), team = tid / quads;  // of threads that share the CTAs to read
+    if (team < teams)
+        for (int i = first + tid % quads; i < first + quads; i += kThreads) {
+            uint4 sum = make_uint4(0, 0, 0, 0);
+            for (int q = team; q < r.size; q += 4 * teams) {  // four loads from other CTAs at a time
+                uint4 part[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                part[j] = q + j < r.size ? *cluster.map_shared_rank(&h.own[code_of(bin)], q + j) : 0;
+                for (int j = 0; j < 4; ++j)
+                    part[j] = q + j * teams < r.size
+                                  ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&h.own[4 * i], q + j * teams))
+                                  : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) c += part[j];
+                for (int j = 0; j < 4; ++j)
+                    sum.x += part[j].x, sum.y += part[j].y, sum.z += part[j].z, sum.w += part[j].w;
+            }
+            uint32_t* bins = &h.all[place(i)];
+            const bool back = 4 * i < kCodes;
+            if (sum.x) atomicAdd(bins + (back ? 3 : 0), sum.x);
+            if (sum.y) atomicAdd(bins + (back ? 2 : 1), sum.y);
+            if (sum.z) atomicAdd(bins + (back ? 1 : 2), sum.z);
+            if (sum.w) atomicAdd(bins + (back ? 0 : 3), sum.w);
         }
-        for (int q = 0; q < r.size; ++q) *cluster.map_shared_rank(&h.all[bin], q) = c;
-    }
+    if (tid == 0) h.all[kTinyBin] = tiny_count;
     u64 own_tiny = 0;
     if (TY == 0) {
         const int tiny = int(h.own[2 * kCodes]);
-        own_tiny = block_reduce(r.sh, Pair{int(threadIdx.x) < tiny ? r.weight(h.tiny[threadIdx.x]) : 0, 0}, add_pairs).a;
-        if (int(threadIdx.x) < r.size) *cluster.map_shared_rank(&h.tiny_mass[r.rank], threadIdx.x) = own_tiny;
+        if (tid < tiny) atomicAdd(&r.sh.bound[0], r.weight(h.tiny[tid]));  // integers: in any order
+    }
+    __syncthreads();
+    if (TY == 0) {
+        own_tiny = r.sh.bound[0];
+        if (tid < r.size) *cluster.map_shared_rank(&h.tiny_mass[r.rank], tid) = own_tiny;
+    }
+    for (int i = tid; i < quads * (r.size - 1); i += kThreads) {
+        const int to = (r.rank + 1 + i / quads) & (r.size - 1), at = place(first + i % quads);
+        *reinterpret_cast<uint4*>(cluster.map_shared_rank(&h.all[at], to)) = *reinterpret_cast<const uint4*>(&h.all[at]);
     }
     cluster.sync();
     return own_tiny;
@@ -717,12 +885,12 @@ __device__ u64 merge_counts(const Row<TY>& r) {
 // logits; such a row goes the general way.
 template <int TY>
 __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, float u, float floor_v, bool greedy,
-                            Partition z) {
+                            uint32_t tiny_count) {
     Shared& sh = r.sh;
     Values& h = sh.values;
     auto cluster = cg::this_cluster();
     const int tid = threadIdx.x;
-    const u64 own_tiny = merge_counts(r);
+    const u64 own_tiny = merge_counts(r, tiny_count);
     const u64 limit = greedy ? 1 : k > 0 && k < a.vocab ? u64(k) : ~u64(0);
     if (greedy) p = 1.f;
 
@@ -753,9 +921,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         push_list(r, fmaxf(TY == 0 && border != kTinyBin ? near_edge(border) : bin_bottom(border), floor_v));
         cluster.sync();
         if (r.rank == 0) {
-            if constexpr (TY == 0)
-                if (a.logprobs) z = partition_of(r);
-            draw_from_list(r, a, row, limit, p, u, 0, z);
+            draw_from_list(r, a, row, limit, p, u, 0);
         }
         return true;
     }
@@ -767,9 +933,18 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         for (int q = 0; q < r.size; ++q) tiny_mass += h.tiny_mass[q];
         u64 weight[kPerThread], mass = 0;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            weight[i] = cnt[i] ? r.weight(near_edge(first + i)) : 0;
-            mass += first + i == kTinyBin ? (cnt[i] ? tiny_mass : 0) : cnt[i] * weight[i];
+        for (int i = 0; i < kPerThread; i += 3) {
+            static_assert(kPerThread % 3 == 0, "three weights at a time");
+            u64 three[3] = {0, 0, 0};
+            if (__any_sync(0xffffffffu, cnt[i] | cnt[i + 1] | cnt[i + 2])) {
+                const float v[3] = {near_edge(first + i), near_edge(first + i + 1), near_edge(first + i + 2)};
+                r.weights(v, three);
+            }
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+                weight[i + j] = cnt[i + j] ? three[j] : 0;
+                mass += first + i + j == kTinyBin ? (cnt[i + j] ? tiny_mass : 0) : cnt[i + j] * weight[i + j];
+            }
         }
         if (p < 1.f) {
             const u64 ahead = block_exclusive(sh, mass);
@@ -796,10 +971,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
             if (sh.found <= kCap) {
                 push_list(r, near_edge(border));
                 cluster.sync();
-                if (r.rank == 0) {
-                    if (a.logprobs) z = partition_of(r);
-                    draw_from_list(r, a, row, limit, p, u, whole, z);
-                }
+                if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, whole);
                 return true;
             }
         }
@@ -831,55 +1003,51 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         const u64 target = drawn(whole, u);
         if (ahead > target || target >= ahead + own.a) return true;
         // the CTA that holds the token
-        if (a.logprobs) z = partition_of(r);
-        r.cut_v = floor_v, r.cut_i = floor_v == -INFINITY ? -1 : INT_MAX;
+        Partition z{1.f, 0.f};
+        if (a.logprobs) z = counted_partition(r);
         if (border == kTinyBin) {
-            r.cut_v = bin_bottom(kTinyBin), r.cut_i = INT_MAX;  // all of the tiny
+            r.keep_from(bin_bottom(kTinyBin));  // all of the tiny
         } else if (border != INT_MAX) {
-            r.cut_v = near_edge(border), r.cut_i = mine ? INT_MAX : -1;
-            if (mine && mine < here) r.cut_i = nth_equal(r, r.cut_v, mine);
+            const float v = near_edge(border);
+            if (mine == here)
+                r.keep_from(v);
+            else if (mine == 0)
+                r.keep_from(nextafterf(v, INFINITY));
+            else
+                r.cut_at(v, nth_equal(r, v, mine));
         }
-        const int turns = (a.vecs + kThreads - 1) / kThreads;
-        slab_masses(r, turns);
+        slab_masses(r);
         __syncthreads();
-        if (tid < 32) write_token(r, a, row, ahead, target, turns, z);
+        if (tid < 32) write_token(r, a, row, ahead, target, z);
         return true;
     } else {
-        r.cut_v = floor_v, r.cut_i = floor_v == -INFINITY ? -1 : INT_MAX;
         // the search below uses the histogram's memory: the counts are in registers, and its own exchanges wait for all
         if (p < 1.f) {
             // Bounds of the bins' masses, and with them of the nucleus' border: it lies in the bins from the
-            // first that can reach it to the first that must.
-            double low = 0.0, high = 0.0;
-            double lower[kPerThread], upper[kPerThread];
+            // first that can reach it to the first that must.  fp32 is enough here: three roundings of an
+            // exponent of at most 37 and sums of some 30 steps are off by less than 1e-5, a quarter of the margins.
+            const float per_t = fminf(float(r.step * (1.0 / (256.0 * 1.4426950408889634074))), 1e37f);
+            float low = 0.f, high = 0.f;
+            float lower[kPerThread], upper[kPerThread];
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                lower[i] = upper[i] = 0.0;
-                if (cnt[i]) {
-                    const float bottom = bin_bottom(first + i), above = bin_top(first + i);
-                    upper[i] = double(cnt[i]) * double(r.weight(fminf(above, r.top)) + 1);
-                    if (bottom >= floor_v) lower[i] = double(cnt[i]) * double(r.weight(bottom));
-                }
+                const float bottom = bin_bottom(first + i), above = fminf(bin_top(first + i), r.top);
+                const float n = float(cnt[i]);
+                upper[i] = cnt[i] ? n * expf(fmaxf((above - r.top) * per_t, -80.f)) : 0.f;
+                lower[i] = cnt[i] && bottom >= floor_v ? n * expf((bottom - r.top) * per_t) : 0.f;
                 low += lower[i], high += upper[i];
             }
-            const Pair ends{u64(__double_as_longlong(low)), u64(__double_as_longlong(high))};
-            const auto add = [](Pair x, Pair y) {
-                return Pair{u64(__double_as_longlong(__longlong_as_double(x.a) + __longlong_as_double(y.a))),
-                            u64(__double_as_longlong(__longlong_as_double(x.b) + __longlong_as_double(y.b)))};
-            };
-            const Pair total = block_reduce(sh, ends, add);
-            const double can = double(p) * __longlong_as_double(total.a) * (1.0 - 1e-9);
-            const double must = double(p) * __longlong_as_double(total.b) * (1.0 + 1e-9);
-            // sums in another order differ in the last bits: the margins above are far wider
-            double at_low = block_exclusive_double(sh, low), at_high = block_exclusive_double(sh, high);
-            if (tid == 0) sh.found_bin = 0, sh.found = kValueBins - 1, sh.bound[0] = 0;
+            const Pair total = block_reduce(sh, Pair{as_bits(low), as_bits(high)}, add_floats);
+            const float can = p * as_float(total.a) * (1.f - 4e-5f), must = p * as_float(total.b) * (1.f + 4e-5f);
+            float at_low, at_high;
+            block_exclusive_floats(sh, low, high, at_low, at_high);
+            if (tid == 0) sh.found_bin = 0, sh.found = kValueBins - 1;
             __syncthreads();
-            u64 c = seen - count;
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                if (at_high < can && can <= at_high + upper[i]) sh.found_bin = first + i;
-                if (at_low < must && must <= at_low + lower[i]) sh.found = first + i;
-                at_high += upper[i], at_low += lower[i], c += cnt[i];
+                if (at_high < can && can <= at_high + upper[i]) atomicMax(&sh.found_bin, first + i);
+                if (at_low < must && must <= at_low + lower[i]) atomicMin(&sh.found, first + i);
+                at_high += upper[i], at_low += lower[i];
             }
             __syncthreads();
             const int open = sh.found_bin, close = sh.found;
@@ -887,49 +1055,23 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
             const u64 counts_open = count_above(sh, first, seen - count, cnt, open);
             const u64 counts_close = count_above(sh, first, seen - count, cnt, close + 1);
             if (by_count) cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
-            const float edge = bin_top(open);
+            const float edge = bin_top(open), above = nextafterf(edge, INFINITY);
             const bool few = counts_close <= u64(kCap) && !by_count;
             if (few) push_list(r, fmaxf(bin_bottom(close), floor_v));
-            u64 mass = 0, above = 0;
-            r.each([&](float x, int slot) {
-                if (r.kept(x, slot)) {
-                    const u64 w = r.weight(x);
-                    mass += w;
-                    if (x > edge) above += w;
-                }
-            });
-            const Pair* all = r.exchange(block_reduce(sh, Pair{mass, above}, add_pairs));
+            const Pair* all = r.exchange(block_reduce(sh, kept_mass(r, above), add_pairs));
             Pair sums{0, 0};
             for (int q = 0; q < r.size; ++q) sums = add_pairs(sums, all[q]);
             if (few) {
-                if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, sums.a, z);
+                if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, sums.a);
                 return true;
             }
             cut_row<TY, true>(r, fmaxf(bin_bottom(close), floor_v), edge, sums.b, nucleus(sums.a, p), counts_close - counts_open);
         } else if (by_count) {
             cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
         }
-        draw_from_row(r, a, row, u, z);
+        draw_from_row(r, a, row, u);
         return true;
     }
-}
-
-// The values of a 16-byte vector of which only a part lies in the row.
-template <int TY>
-__device__ __forceinline__ uint4 edge_vector(const char* begin, int i0, int vocab) {
-    constexpr int E = Elem<TY>::E, kBytes = Elem<TY>::kBytes;
-    uint32_t w[4] = {Elem<TY>::kNone, Elem<TY>::kNone, Elem<TY>::kNone, Elem<TY>::kNone};
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (i0 + e >= 0 && i0 + e < vocab) {
-            if (kBytes == 2) {
-                const uint32_t h = reinterpret_cast<const uint16_t*>(begin)[i0 + e];
-                w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | h << 16 : (w[e / 2] & 0xffff0000u) | h;
-            } else {
-                w[e & 3] = reinterpret_cast<const uint32_t*>(begin)[i0 + e];
-            }
-        }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // One cluster per row.  The barrier of a cluster is the hardware's: all its
@@ -939,8 +1081,9 @@ template <int TY>
 __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     using El = Elem<TY>;
     constexpr int E = El::E, kBatch = 4;
-    extern __shared__ uint4 data[];
-    __shared__ Shared sh;
+    extern __shared__ uint4 dynamic[];
+    Shared& sh = *reinterpret_cast<Shared*>(dynamic);
+    uint4* const data = dynamic + sizeof(Shared) / 16;
     auto cluster = cg::this_cluster();
     cluster.barrier_arrive();  // waited for before the first access to another CTA's shared memory
     const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -953,13 +1096,14 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     const int v0 = min(rank * a.vecs, total_vecs), nvec = min(a.vecs, total_vecs - v0);
     const uint4* base = reinterpret_cast<const uint4*>(begin - lead * El::kBytes) + v0;
     const int i_first = v0 * E - lead;  // index of the first value
+    const bool resident = a.resident;   // the logits stay in shared memory; else later passes find them in L2
     uint4 q[kBatch];
     auto fetch = [&](int b) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const int v = b + j * kThreads + tid, i0 = i_first + v * E;
             if (v < nvec)
-                q[j] = i0 >= 0 && i0 + E <= a.vocab ? __ldcs(base + v) : edge_vector<TY>(begin, i0, a.vocab);
+                q[j] = i0 >= 0 && i0 + E <= a.vocab ? __ldcg(base + v) : edge_vector<TY>(begin, i0, a.vocab);
         }
     };
     fetch(0);
@@ -979,52 +1123,67 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     }
     const bool greedy = T == 0.f || k == 1, cuts = greedy || (k > 0 && k < a.vocab) || p < 1.f;
     const bool counting = TY == 0 || cuts;
+    const double step = greedy ? 0.0 : 256.0 * 1.4426950408889634074 / double(T);
+    const double depth = min_p > 0.f && !greedy ? double(T) * log(double(min_p)) : 0.0;  // of min-p's border
     Values& h = sh.values;
     if (counting) {
-        for (int i = tid; i < kValueBins; i += kThreads) h.own[i] = 0;
-        for (int i = kValueBins + tid; i < kPerThread * kThreads; i += kThreads) h.all[i] = 0;
+        for (int i = tid; i < int(sizeof(h.own) / 16); i += kThreads) reinterpret_cast<uint4*>(h.own)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < int(sizeof(h.all) / 16); i += kThreads) reinterpret_cast<uint4*>(h.all)[i] = make_uint4(0, 0, 0, 0);
     }
-    if (tid < 64) sh.pow64[tid] = exp2(-tid * (1.0 / 64));
-    if (tid == 0) sh.list.n = 0;
+    const int frac = min(51, 62 - (32 - __clz((a.vocab - 1) | 1)));  // s
+    if (tid < 256) sh.pow256[tid] = exp2(frac - tid * (1.0 / 256));
+    if (tid == 0) sh.list.n = 0, sh.bound[0] = 0;
     __syncthreads();
     float top = -INFINITY;
     uint32_t notes = 0;  // 1: NaN or +inf; 2: 128 or more, 4: -128 or less but not -inf, 8: too many tiny
     for (int b = 0; b < nvec; b += kBatch * kThreads) {
-        if (b) fetch(b);
+        uint4 now[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) now[j] = q[j];
+        if (b + kBatch * kThreads < nvec) fetch(b + kBatch * kThreads);  // in flight meanwhile
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const int v = b + j * kThreads + tid;
             if (v >= nvec) break;
-            data[v] = q[j];
+            if (resident) data[v] = now[j];
             float x[E];
-            El::unpack(q[j], x);
+            El::unpack(now[j], x);
+            uint32_t others = 0;  // 1: a value without a code
+            if (counting) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                top = fmaxf(top, x[e]);
-                if (counting) {
-                    const uint32_t bits = __float_as_uint(x[e]) >> 16, magnitude = bits & 0x7fffu;
-                    const uint32_t code = magnitude - kFirstCode;
-                    if (code < uint32_t(kCodes)) {
-                        atomicAdd(&h.own[code + (bits >> 15) * kCodes], 1u);
-                    } else if (magnitude < kFirstCode) {
+                for (int e = 0; e < E; ++e) {
+                    const uint32_t bits = __float_as_uint(x[e]) >> 16;
+                    const uint32_t code = (bits & 0x7fffu) - kFirstCode;
+                    if (code < uint32_t(kCodes)) atomicAdd(&h.own[code + (bits >> 15) * kCodes], 1u);
+                    others |= code >= uint32_t(kCodes);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) others |= !(x[e] < INFINITY);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, x[e]);
+            if (others) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float size_of = fabsf(x[e]);
+                    if (!(x[e] < INFINITY)) {
+                        notes |= 1;
+                    } else if (size_of >= 128.f) {
+                        if (size_of < INFINITY) notes |= x[e] > 0.f ? 2 : 4;
+                    } else if (counting && size_of < 0x1p-10f) {
                         const uint32_t at = atomicAdd(&h.own[2 * kCodes], 1u);
                         if (TY == 0) {
                             if (at < uint32_t(kTinyCap)) h.tiny[at] = x[e];
                             else notes |= 8;
                         }
-                    } else if (!(x[e] < INFINITY)) {
-                        notes |= 1;
-                    } else if (x[e] != -INFINITY) {
-                        notes |= x[e] > 0.f ? 2 : 4;
                     }
-                } else if (!(x[e] < INFINITY)) {
-                    notes |= 1;
                 }
             }
         }
     }
 
-    Row<TY> r{sh, data, nvec, i_first, rank, size, 0};
+    Row<TY> r{sh, resident ? data : nullptr, base, begin, a.vocab, nvec, i_first, rank, size, 0};
     auto join = [](Pair x, Pair y) { return Pair{as_bits(fmaxf(as_float(x.a), as_float(y.a))), x.b | y.b}; };
     const Pair mine = block_reduce(sh, Pair{as_bits(top), notes}, join);
     // sum of exponentials for the log probability, against this CTA's largest logit; a bf16 row takes it from its counts
@@ -1033,17 +1192,22 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         const float local = as_float(mine.a);
         float equal = 0.f, others = 0.f;
         r.each([&](float x, int) {
-            if (x == local)
-                equal += 1.f;
-            else
-                others += expf(__fsub_rn(x, local));
+            const float e = expf(__fsub_rn(x, local));
+            equal += x == local ? 1.f : 0.f;
+            others += x == local ? 0.f : e;
         });
         sums = block_reduce(sh, Pair{as_bits(equal), as_bits(others)}, add_floats);
     }
     cluster.barrier_wait();
-    const Pair* all = r.exchange(Pair{mine.a | mine.b << 32, sums.a | sums.b << 32});
+    const uint32_t own_tiny = counting ? h.own[2 * kCodes] : 0;
+    const Pair* all = r.exchange(Pair{mine.a | (mine.b | own_tiny << 8) << 32, sums.a | sums.b << 32});
+    uint32_t tiny_count = 0;
     top = -INFINITY, notes = 0;
-    for (int i = 0; i < size; ++i) top = fmaxf(top, as_float(all[i].a)), notes |= uint32_t(all[i].a >> 32);
+    for (int i = 0; i < size; ++i) {
+        const uint32_t high = uint32_t(all[i].a >> 32);
+        top = fmaxf(top, as_float(all[i].a)), notes |= high & 255u, tiny_count += high >> 8;
+    }
+    if (TY != 0 && tid < size) sh.part[tid] = all[tid];  // read after a later barrier
     if ((notes & 1) || top == -INFINITY) {
         if (rank == 0 && tid == 0) {
             a.tokens[row] = -1;
@@ -1052,30 +1216,20 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         }
         return;
     }
-    Partition z{0.f, 0.f};
-    if (TY != 0 && a.logprobs)
-        for (int i = 0; i < size; ++i) {
-            const float local = as_float(all[i].a), equal = as_float(all[i].b), others = as_float(all[i].b >> 32);
-            if (local == top)
-                z.tops += equal, z.others += others;
-            else if (local > -INFINITY)
-                z.others = __fmaf_rn(__fadd_rn(equal, others), expf(__fsub_rn(local, top)), z.others);
-        }
     r.top = top;
-    r.step = greedy ? 0.0 : 64.0 * 1.4426950408889634074 / double(T);
-    r.frac = min(51, 62 - (32 - __clz((a.vocab - 1) | 1)));
-    r.count_mode = u == 0.f && !greedy;
+    r.step = step;
+    r.weigh(u == 0.f && !greedy, frac, T);
     // w >= min_p as a comparison of logits, which is exact
     float floor_v = -INFINITY;
-    if (min_p > 0.f && !greedy) floor_v = __double2float_ru(double(top) + double(T) * log(double(min_p)));
-    r.cut_v = floor_v, r.cut_i = floor_v == -INFINITY ? -1 : INT_MAX;
+    if (min_p > 0.f && !greedy) floor_v = __double2float_ru(double(top) + depth);
+    r.keep_from(floor_v);
     if (counting) {
         // The counts must hold every logit that has a weight: below -128 none has from 37 T on.  A bf16 row also
         // needs its largest logit and min-p's border outside the tiny bin, where values are not told apart.
         const float heat = greedy ? 1.f : fmaxf(T, 1.f);
         bool whole = !(notes & 10) && top > -128.f && !r.count_mode && (!(notes & 4) || top + 128.f >= 37.f * heat);
         if (TY == 0) whole = whole && fabsf(top) > bin_top(kTinyBin) && !(fabsf(floor_v) <= bin_top(kTinyBin));
-        if (whole && counted_row(r, a, row, k, p, u, floor_v, greedy, z)) return;
+        if (whole && counted_row(r, a, row, k, p, u, floor_v, greedy, tiny_count)) return;
         cluster.sync();  // the counts' memory is used again
     }
 
@@ -1083,14 +1237,13 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     if (TY == 0 && a.logprobs) {
         float equal = 0.f, others = 0.f;
         r.each([&](float x, int) {
-            if (x == top)
-                equal += 1.f;
-            else
-                others += expf(__fsub_rn(x, top));
+            const float e = expf(__fsub_rn(x, top));
+            equal += x == top ? 1.f : 0.f;
+            others += x == top ? 0.f : e;
         });
         const Pair own = block_reduce(sh, Pair{as_bits(equal), as_bits(others)}, add_floats);
-        all = r.exchange(own);
-        for (int i = 0; i < size; ++i) z.tops += as_float(all[i].a), z.others += as_float(all[i].b);
+        if (tid < size) *cluster.map_shared_rank(&sh.part[rank], tid) = Pair{as_bits(top), own.a | own.b << 32};
+        cluster.sync();
     }
     const bool by_count = greedy || (k > 0 && k < a.vocab), by_mass = p < 1.f && !greedy;
     if (by_count || by_mass) {
@@ -1111,19 +1264,15 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         if (by_count) cut_row<TY, false>(r, from(746.0), top, 0, greedy ? 1 : u64(k), a.vocab);
         if (by_mass) {
             const bool counted = r.count_mode;
-            r.count_mode = false;  // the nucleus goes by mass for u = 0 too
+            r.weigh(false, frac, T);  // the nucleus goes by mass for u = 0 too
+            all = r.exchange(block_reduce(sh, kept_mass(r, top), add_pairs));
             u64 mass = 0;
-            r.each([&](float x, int slot) {
-                if (r.kept(x, slot)) mass += r.weight(x);
-            });
-            all = r.exchange(block_reduce(sh, Pair{mass, 0}, add_pairs));
-            mass = 0;
             for (int i = 0; i < size; ++i) mass += all[i].a;
             cut_row<TY, true>(r, from(37.0), top, 0, nucleus(mass, p), a.vocab);
-            r.count_mode = counted;
+            r.weigh(counted, frac, T);
         }
     }
-    draw_from_row(r, a, row, u, z);
+    draw_from_row(r, a, row, u);
 }
 
 std::atomic<bool> g_attr[3][64];
@@ -1158,11 +1307,11 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     }
     // A row may start inside a 16-byte vector and then takes one more.
     const int total_vecs = (vocab + per_vec - 1 + per_vec - 1) / per_vec;
-    // CTAs a row: so many that a share is at most 64 KB (three or more CTAs fit
-    // an SM), and with few rows as many as give every SM a share of 8 KB or more.
+    // CTAs a row: as many as run at once (two on each SM), as the steps between two passes over the logits take
+    // much the same time for a large share as for a small one; no share below 4 KB, none above kMaxVecs.
     int size = 1;
-    while (size < kMaxCluster && ((total_vecs + size - 1) / size * 16 > 64 * 1024 ||
-                                  (int64_t(M) * size < kSms && total_vecs / size * 16 > 16 * 1024)))
+    while (size < kMaxCluster && ((total_vecs + size - 1) / size > kMaxVecs ||
+                                  (int64_t(M) * size * 2 <= 2 * kSms && total_vecs / size > 512)))
         size *= 2;
     if (int64_t(M) * size > INT_MAX) return cudaErrorInvalidValue;
     NvtxRange range("ornith.sample");
@@ -1175,6 +1324,7 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     a.tokens = static_cast<int32_t*>(tokens), a.logprobs = static_cast<float*>(logprobs);
     a.flags = static_cast<uint32_t*>(flags);
     a.vocab = vocab, a.vecs = (total_vecs + size - 1) / size;
+    a.resident = a.vecs <= (int64_t(M) * size <= kSms ? kAloneVecs : kSharedVecs);
     void (*const kernels[3])(Args) = {sample_kernel<0>, sample_kernel<1>, sample_kernel<2>};
     auto kernel = kernels[type];
     int device = 0;
@@ -1183,7 +1333,7 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
     std::atomic<bool>& done = g_attr[type][device];
     if (!done.load(std::memory_order_acquire)) {
-        st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxVecs + 1) * 16);
+        st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Shared)) + kAloneVecs * 16);
         if (st == cudaSuccess) st = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (st != cudaSuccess) return st;
         done.store(true, std::memory_order_release);
@@ -1191,7 +1341,7 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(M) * unsigned(size));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = size_t(a.vecs) * 16;
+    cfg.dynamicSmemBytes = sizeof(Shared) + (a.resident ? size_t(a.vecs) * 16 : 0);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
