@@ -52,10 +52,11 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kMaxVocab = 1 << 19, kSms = 148;
-constexpr int kBins = 1024, kCap = 256;
-constexpr int kMaxVecs = 1 << 15, kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
+constexpr int kBins = 1024, kCap = 256, kAhead = 4;  // kAhead: vectors of a thread in flight
+constexpr int kMaxVecs = 60 * kThreads, kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
 // 16-byte vectors of a CTA: at most, and kept on chip by one or two CTAs of an SM
-constexpr int kSlabs = kMaxVecs / 32;                        // (turn, warp) pairs of a CTA
+constexpr int kParts = 4;  // of a bf16 CTA's logits that do not stay on chip, counted apart in 16 bits: 15 * kThreads * 8 < 2^16
+constexpr int kStep = 8, kSlabs = kMaxVecs / 32 / kStep + kWarps;  // rows of 32 vectors in a slab; slabs of a CTA
 constexpr float kMaxTemperature = 1e30f;
 constexpr uint32_t kFlagNonfinite = 1, kFlagParameter = 2, kFlagNothingLeft = 4;
 
@@ -69,6 +70,7 @@ struct Args {
     uint32_t* flags;
     int vocab, vecs;  // vecs: 16-byte vectors of a row for one CTA
     int resident;     // they stay in shared memory
+    int part_rows;    // bf16: rows of kThreads vectors in a part that is counted apart, or 0
 };
 
 template <int TY>
@@ -85,6 +87,14 @@ struct Elem<0> {
             x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
+    // the largest value of a vector (of those that are not NaN)
+    static __device__ __forceinline__ float largest(const uint4& v) {
+        uint32_t a, b;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+        asm("max.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+        return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+    }
     static constexpr uint32_t kNone = 0xff80ff80u;  // a vector's word of two -inf
     static constexpr float kLowest = -3.3895313892515355e38f;
 };
@@ -100,6 +110,14 @@ struct Elem<1> {
             x[2 * i + 1] = __half2float(__ushort_as_half(uint16_t(w[i] >> 16)));
         }
     }
+    static __device__ __forceinline__ float largest(const uint4& v) {
+        uint32_t a, b;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+        asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+        asm("max.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+        return fmaxf(__half2float(__ushort_as_half(uint16_t(a & 0xffffu))),
+                     __half2float(__ushort_as_half(uint16_t(a >> 16))));
+    }
     static constexpr uint32_t kNone = 0xfc00fc00u;
     static constexpr float kLowest = -65504.f;
 };
@@ -110,6 +128,10 @@ struct Elem<2> {
     static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[E]) {
         x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y);
         x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ float largest(const uint4& v) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                     fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
     static constexpr uint32_t kNone = 0xff800000u;
     static constexpr float kLowest = -FLT_MAX;
@@ -140,6 +162,7 @@ struct Values {
     alignas(16) uint32_t own[2 * kCodes + 4];      // by code: positive, negative, tiny
     alignas(16) uint32_t all[kPerThread * kThreads];  // the row's, by value
     float tiny[kTinyCap];                          // this CTA's tiny logits (bf16 rows)
+    uint8_t tiny_part[kTinyCap];                   // and where they lie
     u64 tiny_mass[kMaxCluster];                    // pushed
 };
 
@@ -182,19 +205,30 @@ struct alignas(16) Shared {
     List list;
     double pow256[256];                  // 2^(s - j/256)
     Pair slot[2][kMaxCluster];           // pushed by every CTA of the cluster in turn
-    u64 slab[kSlabs];                    // kept mass of each (turn, warp) in index order
+    u64 slab[kSlabs];                    // kept mass of each slab, in index order
     Pair red[kWarps];
     Pair part[kMaxCluster];              // fp16, fp32: every CTA's largest logit, count of it and sum of the others
     u64 bound[2];
+    uint32_t part_here[kParts], part_kept[kParts];  // the border's value in the parts of the token's CTA
     int found, found_bin;
 };
+
+// The dynamic shared memory of a CTA: this, then the vectors that stay on chip.
+extern __shared__ uint4 dynamic[];
+__device__ __forceinline__ Shared& shared() { return *reinterpret_cast<Shared*>(dynamic); }
+__device__ __forceinline__ uint4* vectors() { return dynamic + sizeof(Shared) / 16; }
+// In their place where they do not: counts of part 2i + j in half j of parts()[i * 2 * kCodes + code].
+__device__ __forceinline__ uint32_t* parts() { return reinterpret_cast<uint32_t*>(vectors()); }
+__device__ __forceinline__ uint32_t part_count(int code, int part) {
+    return (parts()[(part >> 1) * 2 * kCodes + code] >> (16 * (part & 1))) & 0xffffu;
+}
 
 __device__ __forceinline__ float as_float(u64 v) { return __uint_as_float(uint32_t(v)); }
 __device__ __forceinline__ u64 as_bits(float v) { return __float_as_uint(v); }
 
 // The values of a 16-byte vector of which only a part lies in the row.
 template <int TY>
-__device__ __forceinline__ uint4 edge_vector(const char* begin, int i0, int vocab) {
+__device__ __noinline__ uint4 edge_vector(const char* begin, int i0, int vocab) {
     constexpr int E = Elem<TY>::E, kBytes = Elem<TY>::kBytes;
     uint32_t w[4] = {Elem<TY>::kNone, Elem<TY>::kNone, Elem<TY>::kNone, Elem<TY>::kNone};
 #pragma unroll
@@ -215,9 +249,9 @@ template <int TY>
 struct Row {
     using El = Elem<TY>;
     static constexpr int E = El::E;
-    Shared& sh;
-    const uint4* data;    // this CTA's vectors in shared memory, or null
-    const uint4* source;  // and where they lie in the tensor
+    bool resident;        // this CTA's vectors are in shared memory
+    int head, tail;       // vectors of which only a part lies in the row, or -1
+    const uint4* source;  // where they lie in the tensor
     const char* begin;    // the row's first logit
     int vocab, nvec, first;  // first: index of slot 0 (below 0 where the row starts inside a vector)
     int rank, size, parity;
@@ -229,26 +263,43 @@ struct Row {
     int tie_i;
 
     __device__ __forceinline__ uint4 vec(int v) const {
-        if (data) return data[v];
-        const int i0 = first + v * E;
-        return i0 >= 0 && i0 + E <= vocab ? __ldcg(source + v) : edge_vector<TY>(begin, i0, vocab);
+        if (resident) return vectors()[v];
+        return v != head && v != tail ? __ldcg(source + v) : edge_vector<TY>(begin, first + v * E, vocab);
     }
     __device__ __forceinline__ bool kept(float x, int slot) const {
         return x >= edge || (x == tie_v && first + slot <= tie_i);
+    }
+    // From here on only vectors [from, from + count).
+    __device__ void narrow(int from, int count) {
+        source += from, first += from * E, nvec = count;
+        head = from == 0 ? head : -1, tail = tail >= from && tail < from + count ? tail - from : -1;
     }
     __device__ void keep_from(float v) { edge = fmaxf(v, -FLT_MAX), tie_v = 0.f, tie_i = -1; }
     __device__ void cut_at(float v, int index) { edge = nextafterf(v, INFINITY), tie_v = v, tie_i = index; }
 
     template <class F>
     __device__ __forceinline__ void each(F f) const {
-        if (int(threadIdx.x) >= nvec) return;
-        uint4 next = vec(threadIdx.x);
-        for (int v = threadIdx.x; v < nvec; v += kThreads) {
+        each_vector([&](int v, const uint4& q) {
             float x[E];
-            El::unpack(next, x);
-            if (v + kThreads < nvec) next = vec(v + kThreads);  // in flight meanwhile
+            El::unpack(q, x);
 #pragma unroll
             for (int e = 0; e < E; ++e) f(x[e], v * E + e);
+        });
+    }
+    template <class F>
+    __device__ __forceinline__ void each_vector(F f) const {
+#pragma unroll 1
+        for (int b = threadIdx.x; b < nvec; b += kAhead * kThreads) {
+            uint4 q[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (b + j * kThreads < nvec) q[j] = vec(b + j * kThreads);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int v = b + j * kThreads;
+                if (v >= nvec) break;
+                f(v, q[j]);
+            }
         }
     }
 
@@ -268,8 +319,8 @@ struct Row {
         double p = __fma_rn(f, -a * a * a / 6, a * a / 2);
         p = __fma_rn(p, f, -a);
         p = __fma_rn(p, f, 1.0);
-        const double v = __dmul_rn(sh.pow256[n & 255], p);
-        const int high = __double2hiint(v) - ((n & ~255) << 12);  // times 2^-(n / 256)
+        const double v = __dmul_rn(shared().pow256[n & 255], p);
+        const int high = __double2hiint(v) + (n & ~255) * -4096;  // times 2^-(n / 256)
         return u64(__double_as_longlong(__dadd_rn(__hiloint2double(in ? high : 0, __double2loint(v)), 0x1p52)));
     }
     static constexpr u64 kRawZero = 0x4330000000000000ull;
@@ -288,27 +339,20 @@ struct Row {
             for (int i = 0; i < N; ++i) w[i] = x[i] >= weigh_from;
         }
     }
-    // The kept mass of vector v, whose values are in q, and, at `above` or higher, a part of it.
-    template <bool PART>
-    __device__ __forceinline__ u64 kept_sum(int v, const uint4& q, float above, u64& part) const {
-        if (v >= nvec) return 0;
+    // Adds the kept mass of vector v, whose values are in q, to `sum` and that at `above` or higher to `part`.
+    // TIES: equal logits lie on both sides of the cut.  No value below `from` is kept.
+    template <bool TIES, bool PART>
+    __device__ __forceinline__ void add_kept(int v, const uint4& q, float from, float above, u64& sum, u64& part) const {
+        if (El::largest(q) < from) return;
         float x[E];
         El::unpack(q, x);
-        bool in[E], any = false;
-        if (tie_i < 0) {  // no equal logits on both sides of the cut: one comparison each
-            const float from = fmaxf(edge, weigh_from);
+        bool in[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) in[e] = x[e] >= from, any |= in[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) in[e] = kept(x[e], v * E + e) && x[e] >= weigh_from, any |= in[e];
-        }
-        if (!any) return 0;
-        u64 sum = 0;
+        for (int e = 0; e < E; ++e) in[e] = TIES ? kept(x[e], v * E + e) && x[e] >= weigh_from : x[e] >= from;
         if (count_mode) {
 #pragma unroll
             for (int e = 0; e < E; ++e) sum += in[e], part += PART && in[e] && x[e] >= above;
-            return sum;
+            return;
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -316,14 +360,30 @@ struct Row {
             sum += raw;
             if (PART) part += x[e] >= above ? raw - kRawZero : 0;
         }
-        return sum - E * kRawZero;
+        sum -= E * kRawZero;
+    }
+    // The vectors of a warp: `steps` rows of 32, so that a slab, kStep of them, is a range of the row.
+    __device__ __forceinline__ int steps() const { return (nvec + 32 * kWarps - 1) / (32 * kWarps); }
+    template <class F>
+    __device__ __forceinline__ void each_step(F f) const {
+        const int n = steps(), from = (int(threadIdx.x) >> 5) * n * 32 + int(threadIdx.x & 31);
+#pragma unroll 1
+        for (int s = 0; s < n; s += kAhead) {
+            uint4 q[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (s + j < n && from + 32 * (s + j) < nvec) q[j] = vec(from + 32 * (s + j));
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (s + j < n) f(s + j, from + 32 * (s + j), q[j]);
+        }
     }
 
     // Everyone's pair, in rank order, after all have pushed theirs.  The two
     // buffers alternate: a CTA writes a buffer again only after a later
     // exchange, which its readers join when they have read it.
     __device__ const Pair* exchange(const Pair& mine) {
-        Pair* box = sh.slot[parity];
+        Pair* box = shared().slot[parity];
         auto cluster = cg::this_cluster();
         if (int(threadIdx.x) < size) *cluster.map_shared_rank(box + rank, threadIdx.x) = mine;
         cluster.sync();
@@ -333,7 +393,8 @@ struct Row {
 };
 
 template <class Op>
-__device__ __forceinline__ Pair block_reduce(Shared& sh, Pair v, Op op) {
+__device__ __forceinline__ Pair block_reduce(Pair v, Op op) {
+    Shared& sh = shared();
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
         const Pair o{__shfl_xor_sync(0xffffffffu, v.a, d), __shfl_xor_sync(0xffffffffu, v.b, d)};
@@ -342,9 +403,12 @@ __device__ __forceinline__ Pair block_reduce(Shared& sh, Pair v, Op op) {
     __syncthreads();  // red may still be read from the call before
     if ((threadIdx.x & 31) == 0) sh.red[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = sh.red[0];
+    v = sh.red[threadIdx.x & (kWarps - 1)];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) v = op(v, sh.red[w]);
+    for (int d = kWarps / 2; d > 0; d >>= 1) {
+        const Pair o{__shfl_xor_sync(0xffffffffu, v.a, d), __shfl_xor_sync(0xffffffffu, v.b, d)};
+        v = op(v, o);
+    }
     return v;
 }
 
@@ -359,7 +423,8 @@ __device__ __forceinline__ u64 warp_exclusive(u64 v) {
 }
 
 // Exclusive prefix of one value per thread over the block.
-__device__ __forceinline__ u64 block_exclusive(Shared& sh, u64 v) {
+__device__ __forceinline__ u64 block_exclusive(u64 v) {
+    Shared& sh = shared();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const u64 prior = warp_exclusive(v);
     __syncthreads();
@@ -372,29 +437,32 @@ __device__ __forceinline__ u64 block_exclusive(Shared& sh, u64 v) {
     return before + prior;
 }
 
-// Exclusive prefixes of two floats per thread over the block.
-__device__ void block_exclusive_floats(Shared& sh, float a, float b, float& before_a, float& before_b) {
+// Exclusive prefix of a float per thread over the block, and the sum of all.
+__device__ __forceinline__ void block_exclusive_float(float v, float& before, float& total) {
+    Shared& sh = shared();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float ia = a, ib = b;
+    float inc = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const float oa = __shfl_up_sync(0xffffffffu, ia, d), ob = __shfl_up_sync(0xffffffffu, ib, d);
-        if (lane >= d) ia += oa, ib += ob;
+        const float o = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += o;
     }
     __syncthreads();
-    if (lane == 31) sh.red[warp] = Pair{u64(__float_as_uint(ia)), u64(__float_as_uint(ib))};
+    if (lane == 31) sh.red[warp].a = u64(__float_as_uint(inc));
     __syncthreads();
-    before_a = __shfl_up_sync(0xffffffffu, ia, 1), before_b = __shfl_up_sync(0xffffffffu, ib, 1);
-    if (lane == 0) before_a = before_b = 0.f;
-    float wa = 0.f, wb = 0.f;
+    before = __shfl_up_sync(0xffffffffu, inc, 1);
+    if (lane == 0) before = 0.f;
+    total = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-        if (w < warp) wa += __uint_as_float(uint32_t(sh.red[w].a)), wb += __uint_as_float(uint32_t(sh.red[w].b));
-    before_a += wa, before_b += wb;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) before += total;
+        total += __uint_as_float(uint32_t(sh.red[w].a));
+    }
 }
 
 // Tokens in the bins before `bin`, from counts that lie kPerThread to a thread.
-__device__ u64 count_above(Shared& sh, int first, u64 before, const uint32_t (&cnt)[kPerThread], int bin) {
+__device__ u64 count_above(int first, u64 before, const uint32_t (&cnt)[kPerThread], int bin) {
+    Shared& sh = shared();
     __syncthreads();
     if (first <= bin && bin < first + kPerThread) {
         u64 c = before;
@@ -415,9 +483,12 @@ __device__ __forceinline__ u64 ceil_div(u64 n, u64 d) {
     return q;
 }
 
-// Sums of slabs (turn, warp), in index order -> the slab that running sum
-// `target` falls into and the sum before it.  For one warp.
-__device__ __forceinline__ int find_slab(const Shared& sh, int slabs, u64 target, u64& sum) {
+__device__ __forceinline__ int slabs_of_warp(int steps) { return (steps + kStep - 1) / kStep; }
+
+// Sums of slabs, in index order -> the slab that running sum `target` falls
+// into and the sum before it.  For one warp.
+__device__ __forceinline__ int find_slab(int slabs, u64 target, u64& sum) {
+    const Shared& sh = shared();
     const int lane = threadIdx.x & 31, per_lane = (slabs + 31) / 32;
     int slab = min(lane * per_lane, slabs);
     const int end = min(slab + per_lane, slabs);
@@ -431,8 +502,54 @@ __device__ __forceinline__ int find_slab(const Shared& sh, int slabs, u64 target
     slab = __shfl_sync(0xffffffffu, slab, from), sum = __shfl_sync(0xffffffffu, sum, from);
     return slab;
 }
-__device__ __forceinline__ int slab_vector(int slab) {  // of a lane of the slab's warp
-    return (slab / kWarps) * kThreads + (slab % kWarps) * 32 + int(threadIdx.x & 31);
+
+// The value whose weight (weigh(x, slot)) running sum `target` falls into,
+// `ahead` before this CTA's slabs; found(x, slot) by one thread.  Every warp
+// finds the slab, a warp adds up each of its steps, and the first warp goes
+// through the step.
+template <int TY, class W, class F>
+__device__ __forceinline__ void find_value(const Row<TY>& r, u64 ahead, u64 target, W weigh, F found) {
+    constexpr int E = Elem<TY>::E;
+    static_assert(kStep <= kWarps, "a warp for each step");
+    Shared& sh = shared();
+    const int n = r.steps(), each = slabs_of_warp(n), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int slab = find_slab(kWarps * each, target, ahead), first = slab / each * n, from = first + slab % each * kStep;
+    const auto step_mass = [&](int step, u64 (&w)[E], float (&x)[E]) {
+        const int v = step * 32 + lane;
+        u64 vec = 0;
+        if (v < r.nvec) Elem<TY>::unpack(r.vec(v), x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            w[e] = v < r.nvec ? weigh(x[e], v * E + e) : 0;
+            vec += w[e];
+        }
+        return vec;
+    };
+    u64 w[E] = {};
+    float x[E];
+    if (warp < kStep) {
+        u64 sum = from + warp < first + n ? step_mass(from + warp, w, x) : 0;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) sh.red[warp].a = sum;
+    }
+    __syncthreads();
+    int step = 0;
+    while (step < kStep - 1 && ahead + sh.red[step].a <= target) ahead += sh.red[step++].a;
+    if (warp == step) {  // it has the values at hand
+        u64 vec = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) vec += w[e];
+        u64 at = ahead + warp_exclusive(vec);
+        if (at <= target && target < at + vec) {
+            bool done = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                at += w[e];
+                if (!done && at > target) found(x[e], ((from + step) * 32 + lane) * E + e), done = true;
+            }
+        }
+    }
 }
 
 // The index of this CTA's `nth` kept token (from 1) whose logit is `value`; -1
@@ -440,39 +557,28 @@ __device__ __forceinline__ int slab_vector(int slab) {  // of a lane of the slab
 template <int TY>
 __device__ int nth_equal(const Row<TY>& r, float value, u64 nth) {
     constexpr int E = Elem<TY>::E;
-    Shared& sh = r.sh;
-    const int turns = (r.nvec + kThreads - 1) / kThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const auto ties = [&](int v, bool (&tie)[E]) {
-        float x[E];
-        if (v < r.nvec) Elem<TY>::unpack(r.vec(v), x);
-        uint32_t n = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            tie[e] = v < r.nvec && x[e] == value && r.kept(x[e], v * E + e);
-            n += tie[e];
-        }
-        return n;
-    };
+    Shared& sh = shared();
+    const int n = r.steps(), each = slabs_of_warp(n), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __syncthreads();  // slab may still be read
     if (threadIdx.x == 0) sh.found_bin = -1;
-    for (int turn = 0; turn < turns; ++turn) {
-        bool tie[E];
-        const uint32_t n = __reduce_add_sync(0xffffffffu, ties(turn * kThreads + int(threadIdx.x), tie));
-        if (lane == 0) sh.slab[turn * kWarps + warp] = n;
-    }
-    __syncthreads();
-    if (warp == 0 && nth > 0 && turns > 0) {
-        u64 sum = 0;
-        const int v = slab_vector(find_slab(sh, turns * kWarps, nth - 1, sum));
-        bool tie[E];
-        const uint32_t n = ties(v, tie);
-        u64 at = sum + warp_exclusive(n);
-        if (at < nth && nth <= at + n) {
+    uint32_t ties = 0;
+    r.each_step([&](int s, int v, const uint4& q) {
+        if (v < r.nvec && Elem<TY>::largest(q) >= value) {
+            float x[E];
+            Elem<TY>::unpack(q, x);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (tie[e] && ++at == nth) sh.found_bin = r.first + v * E + e;
+            for (int e = 0; e < E; ++e) ties += x[e] == value && r.kept(value, v * E + e);
         }
-    }
+        if (s % kStep == kStep - 1 || s == n - 1) {
+            ties = __reduce_add_sync(0xffffffffu, ties);
+            if (lane == 0) sh.slab[warp * each + s / kStep] = ties;
+            ties = 0;
+        }
+    });
+    __syncthreads();
+    if (nth > 0 && n > 0)
+        find_value(r, 0, nth - 1, [&](float x, int slot) { return u64(x == value && r.kept(value, slot)); },
+                   [&](float, int slot) { sh.found_bin = r.first + slot; });
     __syncthreads();
     return sh.found_bin;
 }
@@ -483,7 +589,7 @@ __device__ int nth_equal(const Row<TY>& r, float value, u64 nth) {
 // Every CTA of the cluster takes the same decisions from the same merged sums.
 template <int TY, bool MASS>
 __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u64 n) {
-    Shared& sh = r.sh;
+    Shared& sh = shared();
     Search& f = sh.search;
     auto cluster = cg::this_cluster();
     const int per = kBins / r.size;  // bins that one CTA merges
@@ -502,7 +608,7 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
         auto range = [](Pair p, Pair q) {
             return Pair{as_bits(fminf(as_float(p.a), as_float(q.a))), as_bits(fmaxf(as_float(p.b), as_float(q.b)))};
         };
-        Pair own = block_reduce(sh, Pair{as_bits(mn), as_bits(mx)}, range);
+        Pair own = block_reduce(Pair{as_bits(mn), as_bits(mx)}, range);
         const Pair* all = r.exchange(own);
         for (int q = 0; q < r.size; ++q) own = range(own, all[q]);
         lo = as_float(own.a), hi = as_float(own.b), border = -1;
@@ -518,7 +624,7 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
             u64 ties = 0;
             r.each([&](float x, int slot) { ties += inside(x, slot); });
             auto add = [](Pair p, Pair q) { return Pair{p.a + q.a, 0}; };
-            all = r.exchange(block_reduce(sh, Pair{ties, 0}, add));
+            all = r.exchange(block_reduce(Pair{ties, 0}, add));
             u64 ahead = 0;
             for (int q = 0; q < r.rank; ++q) ahead += all[q].a;
             const int mine = nth_equal(r, hi, ahead < need ? need - ahead : 0);
@@ -530,8 +636,8 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
         }
         scale = __fdiv_rn(float(kBins), __fsub_rn(hi, lo));
         for (int b = threadIdx.x; b < kBins; b += kThreads) {
-            f.cnt[b] = 0;
-            if (MASS) f.mass[b] = 0;
+            f.cnt[b] = f.tcnt[b] = 0;
+            if (MASS) f.mass[b] = f.tmass[b] = 0;
         }
         if (threadIdx.x == 0) sh.found = 0;
         __syncthreads();
@@ -543,24 +649,31 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
             }
         });
         cluster.sync();
-        for (int i = threadIdx.x; i < per; i += kThreads) {
-            const int b = r.rank * per + i;
-            uint32_t c = 0;
-            u64 w = 0;
-            for (int q = 0; q < r.size; ++q) {
-                c += *cluster.map_shared_rank(&f.cnt[b], q);
-                if (MASS) w += *cluster.map_shared_rank(&f.mass[b], q);
+        // this CTA's range of bins, by teams of threads that share the CTAs to read
+        const int teams = max(1, kThreads / per), team = int(threadIdx.x) / per;
+        if (team < teams)
+            for (int i = int(threadIdx.x) % per; i < per; i += kThreads) {
+                const int b = r.rank * per + i;
+                uint32_t c = 0;
+                u64 w = 0;
+                for (int q = team; q < r.size; q += teams) {
+                    c += *cluster.map_shared_rank(&f.cnt[b], q);
+                    if (MASS) w += *cluster.map_shared_rank(&f.mass[b], q);
+                }
+                if (c) atomicAdd(&f.tcnt[b], c);
+                if (MASS && w) atomicAdd(&f.tmass[b], w);
             }
-            for (int q = 0; q < r.size; ++q) {
-                *cluster.map_shared_rank(&f.tcnt[b], q) = c;
-                if (MASS) *cluster.map_shared_rank(&f.tmass[b], q) = w;
-            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < per * (r.size - 1); i += kThreads) {
+            const int to = (r.rank + 1 + i / per) & (r.size - 1), b = r.rank * per + i % per;
+            *cluster.map_shared_rank(&f.tcnt[b], to) = f.tcnt[b];
+            if (MASS) *cluster.map_shared_rank(&f.tmass[b], to) = f.tmass[b];
         }
         cluster.sync();
         // two bins a thread, from the largest values down
         const int b0 = 2 * threadIdx.x;
         const u64 v0 = MASS ? f.tmass[b0] : f.tcnt[b0], v1 = MASS ? f.tmass[b0 + 1] : f.tcnt[b0 + 1];
-        const u64 at = base + block_exclusive(sh, v0 + v1);
+        const u64 at = base + block_exclusive(v0 + v1);
         if (at < target && target <= at + v0) sh.found_bin = b0, sh.bound[1] = at, sh.found = 1;
         if (at + v0 < target && target <= at + v0 + v1) sh.found_bin = b0 + 1, sh.bound[1] = at + v0, sh.found = 1;
         __syncthreads();
@@ -605,7 +718,7 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
     }
     __syncthreads();
     const u64 w = mine ? f.gw[threadIdx.x] : 0;
-    const u64 sum = base + block_exclusive(sh, w);
+    const u64 sum = base + block_exclusive(w);
     if (sum < target && target <= sum + w) sh.found_bin = threadIdx.x, sh.found = 1;  // its place
     __syncthreads();
     const bool found = sh.found;
@@ -615,41 +728,44 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
     __syncthreads();
 }
 
-// The kept mass of each (turn, warp) of this CTA into sh.slab, and its sum.
-// Vectors v = turn * kThreads + thread of a warp are consecutive in the row,
-// so slabs in order are in index order.
+// The kept mass of each slab of this CTA into sh.slab, and their sum.
+template <int TY, bool TIES>
+__device__ u64 slab_masses(const Row<TY>& r) {
+    const int n = r.steps(), each = slabs_of_warp(n), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float from = fmaxf(TIES ? r.tie_v : r.edge, r.weigh_from);
+    u64 mine = 0, sum = 0, unused = 0;
+    __syncthreads();  // slab may still be read
+    r.each_step([&](int s, int v, const uint4& q) {
+        if (v < r.nvec) r.template add_kept<TIES, false>(v, q, from, 0.f, sum, unused);
+        if (s % kStep == kStep - 1 || s == n - 1) {
+            if (__any_sync(0xffffffffu, sum != 0)) {
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            }
+            if (lane == 0) shared().slab[warp * each + s / kStep] = sum;
+            mine += sum, sum = 0;
+        }
+    });
+    return lane == 0 ? mine : 0;
+}
 template <int TY>
 __device__ u64 slab_masses(const Row<TY>& r) {
-    const int turns = (r.nvec + kThreads - 1) / kThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    u64 mine = 0, unused = 0;
-    __syncthreads();  // slab may still be read
-    uint4 next = int(threadIdx.x) < r.nvec ? r.vec(threadIdx.x) : uint4{};
-    for (int turn = 0; turn < turns; ++turn) {
-        const uint4 q = next;
-        const int v = turn * kThreads + int(threadIdx.x);
-        if (v + kThreads < r.nvec) next = r.vec(v + kThreads);  // in flight meanwhile
-        u64 sum = r.template kept_sum<false>(v, q, 0.f, unused);
-        if (__any_sync(0xffffffffu, sum != 0)) {
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        }
-        if (lane == 0) r.sh.slab[turn * kWarps + warp] = sum;
-        mine += sum;
-    }
-    return lane == 0 ? mine : 0;
+    return r.tie_i < 0 ? slab_masses<TY, false>(r) : slab_masses<TY, true>(r);
 }
 
 // The kept mass of this CTA, and that at `above` or higher, in this thread's vectors.
 template <int TY>
 __device__ Pair kept_mass(const Row<TY>& r, float above) {
     Pair sum{0, 0};
-    uint4 next = int(threadIdx.x) < r.nvec ? r.vec(threadIdx.x) : uint4{};
-#pragma unroll 1
-    for (int v = threadIdx.x; v < r.nvec; v += kThreads) {
-        const uint4 q = next;
-        if (v + kThreads < r.nvec) next = r.vec(v + kThreads);  // in flight meanwhile
-        sum.a += r.template kept_sum<true>(v, q, above, sum.b);
-    }
+    const bool ties = r.tie_i >= 0;
+    const float from = fmaxf(ties ? r.tie_v : r.edge, r.weigh_from);
+    r.each_step([&](int, int v, const uint4& q) {
+        if (v >= r.nvec) return;
+        if (ties)
+            r.template add_kept<true, true>(v, q, from, above, sum.a, sum.b);
+        else
+            r.template add_kept<false, true>(v, q, from, above, sum.a, sum.b);
+    });
     return sum;
 }
 
@@ -662,34 +778,14 @@ struct Partition {
     }
 };
 
-// One warp of the CTA that holds the token: its slab, its lane, its value.
+// For the CTA that holds the token.
 template <int TY>
 __device__ void write_token(const Row<TY>& r, const Args& a, int row, u64 ahead, u64 target, const Partition& z) {
-    constexpr int E = Elem<TY>::E;
-    const int turns = (r.nvec + kThreads - 1) / kThreads;
-    u64 at = ahead;
-    const int v = slab_vector(find_slab(r.sh, turns * kWarps, target, at));
-    float x[E];
-    u64 w[E], vec = 0;
-    if (v < r.nvec) Elem<TY>::unpack(r.vec(v), x);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        w[e] = v < r.nvec && r.kept(x[e], v * E + e) ? r.weight(x[e]) : 0;
-        vec += w[e];
-    }
-    at += warp_exclusive(vec);
-    if (at <= target && target < at + vec) {
-        bool done = false;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            at += w[e];
-            if (!done && at > target) {
-                a.tokens[row] = r.first + v * E + e;
-                if (a.logprobs) a.logprobs[row] = z.of(x[e], r.top);
-                done = true;
-            }
-        }
-    }
+    find_value(r, ahead, target, [&](float x, int slot) { return r.kept(x, slot) ? r.weight(x) : 0; },
+               [&](float x, int slot) {
+                   a.tokens[row] = r.first + slot;
+                   if (a.logprobs) a.logprobs[row] = z.of(x, r.top);
+               });
 }
 
 __device__ __forceinline__ Pair add_floats(Pair p, Pair q) {
@@ -712,7 +808,7 @@ __device__ Partition joined_partition(const Row<TY>& r) {
     Partition z{0.f, 0.f};
     const int lane = threadIdx.x & 31;
     if (lane < r.size) {
-        const Pair part = r.sh.part[lane];
+        const Pair part = shared().part[lane];
         const float local = as_float(part.a), equal = as_float(part.b), others = as_float(part.b >> 32);
         if (local == r.top)
             z = Partition{equal, others};
@@ -729,7 +825,7 @@ __device__ Partition joined_partition(const Row<TY>& r) {
 
 // The same in a bf16 row's counts, for a block.
 __device__ Partition counted_partition(const Row<0>& r) {
-    const Values& h = r.sh.values;
+    const Values& h = shared().values;
     float others = 0.f, tops = 0.f;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
@@ -741,7 +837,7 @@ __device__ Partition counted_partition(const Row<0>& r) {
             others = v == r.top ? others : __fmaf_rn(c, e, others);
         }
     }
-    const Pair sums = block_reduce(r.sh, Pair{as_bits(tops), as_bits(others)}, add_floats);
+    const Pair sums = block_reduce(Pair{as_bits(tops), as_bits(others)}, add_floats);
     return Partition{as_float(sums.a), as_float(sums.b)};
 }
 
@@ -750,12 +846,17 @@ __device__ Partition counted_partition(const Row<0>& r) {
 template <int TY>
 __device__ void push_list(const Row<TY>& r, float bottom) {
     auto cluster = cg::this_cluster();
-    List& l = *cluster.map_shared_rank(&r.sh.list, 0);
-    r.each([&](float x, int slot) {
-        if (x >= bottom) {
-            const uint32_t at = atomicAdd(&l.n, 1u);
-            if (at < uint32_t(kCap)) l.v[at] = x, l.i[at] = r.first + slot;
-        }
+    List& l = *cluster.map_shared_rank(&shared().list, 0);
+    r.each_vector([&](int v, const uint4& q) {
+        if (Elem<TY>::largest(q) < bottom) return;
+        float x[Elem<TY>::E];
+        Elem<TY>::unpack(q, x);
+#pragma unroll
+        for (int e = 0; e < Elem<TY>::E; ++e)
+            if (x[e] >= bottom) {
+                const uint32_t at = atomicAdd(&l.n, 1u);
+                if (at < uint32_t(kCap)) l.v[at] = x[e], l.i[at] = r.first + v * Elem<TY>::E + e;
+            }
     });
 }
 
@@ -763,7 +864,7 @@ __device__ void push_list(const Row<TY>& r, float bottom) {
 // `whole`: the mass that top-p refers to; 0: that of the first `limit`.
 template <int TY>
 __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 limit, float p, float u, u64 whole) {
-    Shared& sh = r.sh;
+    Shared& sh = shared();
     List& l = sh.list;
     const int tid = threadIdx.x, n = min(int(l.n), kCap);
     Partition z{1.f, 0.f};
@@ -788,7 +889,7 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
     __syncthreads();
     u64 w = tid < n ? l.weight[tid] : 0;
     if (p < 1.f) {
-        const u64 before = block_exclusive(sh, w);
+        const u64 before = block_exclusive(w);
         if (tid == kThreads - 1) sh.bound[0] = before + w;
         __syncthreads();
         const u64 target = nucleus(whole ? whole : sh.bound[0], p);
@@ -796,7 +897,7 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
         __syncthreads();
     }
     const int keep = sh.found_bin + 1;
-    const u64 mass = block_reduce(sh, Pair{tid < keep ? w : 0, 0}, add_pairs).a;
+    const u64 mass = block_reduce(Pair{tid < keep ? w : 0, 0}, add_pairs).a;
     const u64 target = drawn(mass, u);
     // mass up to each kept token in index order
     w = 0;
@@ -813,10 +914,11 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
     }
 }
 
-// Kept masses of the CTAs -> the one that holds the token finds it.
+// Kept masses of the CTAs -> the one that holds the token finds it.  unit: where
+// that mass times it is the sum of exponentials for the log probability; else 0.
 template <int TY>
-__device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u) {
-    const Pair own = block_reduce(r.sh, Pair{slab_masses(r), 0}, add_pairs);
+__device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, float unit) {
+    const Pair own = block_reduce(Pair{slab_masses(r), 0}, add_pairs);
     const Pair* all = r.exchange(own);
     u64 whole = 0, ahead = 0;
     for (int q = 0; q < r.size; ++q) {
@@ -824,8 +926,11 @@ __device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u) {
         whole += all[q].a;
     }
     const u64 target = drawn(whole, u);
-    if (ahead <= target && target < ahead + own.a && threadIdx.x < 32)
-        write_token(r, a, row, ahead, target, a.logprobs ? joined_partition(r) : Partition{1.f, 0.f});
+    if (ahead <= target && target < ahead + own.a)
+        write_token(r, a, row, ahead, target,
+                    unit != 0.f      ? Partition{1.f, float(double(whole) * unit - 1.0)}
+                    : a.logprobs ? joined_partition(r)
+                                     : Partition{1.f, 0.f});
 }
 
 // The row's counts, by value, in every CTA; and for bf16 the mass of the tiny.
@@ -833,14 +938,14 @@ __device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u) {
 // result, and pushes that to the others.
 template <int TY>
 __device__ u64 merge_counts(const Row<TY>& r, uint32_t tiny_count) {
-    Values& h = r.sh.values;
+    Values& h = shared().values;
     auto cluster = cg::this_cluster();
     const int tid = threadIdx.x, quads = 2 * kCodes / 4 / r.size, first = r.rank * quads;
     const auto place = [](int quad) {  // the bins of codes 4 * quad + {0..3}: backwards for the positive ones
         return 4 * quad < kCodes ? kCodes - 4 - 4 * quad : kNegative + 4 * quad - kCodes;
     };
     const int teams = max(1, kThreads / quads), team = tid / quads;  // of threads that share the CTAs to read
-    if (team < teams)
+    if (r.size > 1 && team < teams)
         for (int i = first + tid % quads; i < first + quads; i += kThreads) {
             uint4 sum = make_uint4(0, 0, 0, 0);
             for (int q = team; q < r.size; q += 4 * teams) {  // four loads from other CTAs at a time
@@ -861,15 +966,18 @@ __device__ u64 merge_counts(const Row<TY>& r, uint32_t tiny_count) {
             if (sum.z) atomicAdd(bins + (back ? 1 : 2), sum.z);
             if (sum.w) atomicAdd(bins + (back ? 0 : 3), sum.w);
         }
+    if (r.size == 1)
+        for (int i = tid; i < 2 * kCodes; i += kThreads)
+            h.all[i < kCodes ? kCodes - 1 - i : i - kCodes + kNegative] = h.own[i];
     if (tid == 0) h.all[kTinyBin] = tiny_count;
     u64 own_tiny = 0;
     if (TY == 0) {
         const int tiny = int(h.own[2 * kCodes]);
-        if (tid < tiny) atomicAdd(&r.sh.bound[0], r.weight(h.tiny[tid]));  // integers: in any order
+        if (tid < tiny) atomicAdd(&shared().bound[0], r.weight(h.tiny[tid]));  // integers: in any order
     }
     __syncthreads();
     if (TY == 0) {
-        own_tiny = r.sh.bound[0];
+        own_tiny = shared().bound[0];
         if (tid < r.size) *cluster.map_shared_rank(&h.tiny_mass[r.rank], tid) = own_tiny;
     }
     for (int i = tid; i < quads * (r.size - 1); i += kThreads) {
@@ -886,7 +994,7 @@ __device__ u64 merge_counts(const Row<TY>& r, uint32_t tiny_count) {
 template <int TY>
 __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, float u, float floor_v, bool greedy,
                             uint32_t tiny_count) {
-    Shared& sh = r.sh;
+    Shared& sh = shared();
     Values& h = sh.values;
     auto cluster = cg::this_cluster();
     const int tid = threadIdx.x;
@@ -904,7 +1012,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         count += cnt[i];
     }
     if (tid == 0) sh.found = 0;
-    u64 seen = block_exclusive(sh, count);
+    u64 seen = block_exclusive(count);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
         if (seen < limit && limit <= seen + cnt[i])
@@ -947,7 +1055,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
             }
         }
         if (p < 1.f) {
-            const u64 ahead = block_exclusive(sh, mass);
+            const u64 ahead = block_exclusive(mass);
             if (tid == kThreads - 1) sh.bound[0] = ahead + mass;
             __syncthreads();
             const u64 whole = sh.bound[0], target = nucleus(whole, p);
@@ -993,7 +1101,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
                 mass += (bin == border ? mine : h.own[code_of(bin)]) * weight[i];
         }
         if (tid == 0 && border >= kTinyBin && floor_v <= 0.f) mass += own_tiny;
-        const Pair own = block_reduce(sh, Pair{mass, 0}, add_pairs);
+        const Pair own = block_reduce(Pair{mass, 0}, add_pairs);
         const Pair* all = r.exchange(own);
         u64 whole = 0, ahead = 0;
         for (int q = 0; q < r.size; ++q) {
@@ -1005,6 +1113,47 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         // the CTA that holds the token
         Partition z{1.f, 0.f};
         if (a.logprobs) z = counted_partition(r);
+        u64 target_at = ahead;
+        if (a.part_rows) {
+            // the part that holds it, by the parts' counts
+            u64 of[kParts] = {0, 0, 0, 0};
+#pragma unroll 1
+            for (int i = 0; i < kPerThread; ++i) {
+                const int bin = first + i;
+                if (bin == border) {
+                    u64 left = mine;
+                    for (int q = 0; q < kParts; ++q) {
+                        const uint32_t c = bin == kTinyBin ? 0 : part_count(code_of(bin), q);
+                        const u64 keep = min(left, u64(c));
+                        sh.part_here[q] = c, sh.part_kept[q] = uint32_t(keep), left -= keep;
+                    }
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int bin = first + i;
+                if (bin != kTinyBin && weight[i] && bin <= border) {
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q)
+                        of[q] += (bin == border ? sh.part_kept[q] : part_count(code_of(bin), q)) * weight[i];
+                }
+            }
+            if (border >= kTinyBin && floor_v <= 0.f && tid < int(h.own[2 * kCodes])) {
+                const u64 w = r.weight(h.tiny[tid]);
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) of[q] += h.tiny_part[tid] == q ? w : 0;
+            }
+            const Pair front = block_reduce(Pair{of[0], of[1]}, add_pairs), back = block_reduce(Pair{of[2], of[3]}, add_pairs);
+            const u64 sums[kParts] = {front.a, front.b, back.a, back.b};
+            int part = 0;
+#pragma unroll
+            for (int q = 0; q < kParts - 1; ++q)
+                if (part == q && target_at + sums[q] <= target) target_at += sums[q], part = q + 1;
+            const int from = part * a.part_rows * kThreads;
+            r.narrow(from, min(a.part_rows * kThreads, r.nvec - from));
+            if (border != INT_MAX) here = sh.part_here[part], mine = sh.part_kept[part];
+        }
         if (border == kTinyBin) {
             r.keep_from(bin_bottom(kTinyBin));  // all of the tiny
         } else if (border != INT_MAX) {
@@ -1018,60 +1167,99 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         }
         slab_masses(r);
         __syncthreads();
-        if (tid < 32) write_token(r, a, row, ahead, target, z);
+        write_token(r, a, row, target_at, target, z);
         return true;
     } else {
         // the search below uses the histogram's memory: the counts are in registers, and its own exchanges wait for all
         if (p < 1.f) {
-            // Bounds of the bins' masses, and with them of the nucleus' border: it lies in the bins from the
-            // first that can reach it to the first that must.  fp32 is enough here: three roundings of an
-            // exponent of at most 37 and sums of some 30 steps are off by less than 1e-5, a quarter of the margins.
+            // The bins' masses by their middle values are some per mille off, so the border almost always lies in
+            // the bins from 1.5% of the mass before its estimate to 1.5% after; the exact masses below tell.
             const float per_t = fminf(float(r.step * (1.0 / (256.0 * 1.4426950408889634074))), 1e37f);
-            float low = 0.f, high = 0.f;
-            float lower[kPerThread], upper[kPerThread];
+            float estimate = 0.f, masses[kPerThread];
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                const float bottom = bin_bottom(first + i), above = fminf(bin_top(first + i), r.top);
-                const float n = float(cnt[i]);
-                upper[i] = cnt[i] ? n * expf(fmaxf((above - r.top) * per_t, -80.f)) : 0.f;
-                lower[i] = cnt[i] && bottom >= floor_v ? n * expf((bottom - r.top) * per_t) : 0.f;
-                low += lower[i], high += upper[i];
+                const float middle = fminf(0.5f * bin_bottom(first + i) + 0.5f * bin_top(first + i), r.top);
+                masses[i] = cnt[i] ? float(cnt[i]) * expf((middle - r.top) * per_t) : 0.f;
+                estimate += masses[i];
             }
-            const Pair total = block_reduce(sh, Pair{as_bits(low), as_bits(high)}, add_floats);
-            const float can = p * as_float(total.a) * (1.f - 4e-5f), must = p * as_float(total.b) * (1.f + 4e-5f);
-            float at_low, at_high;
-            block_exclusive_floats(sh, low, high, at_low, at_high);
+            float at, total;
+            block_exclusive_float(estimate, at, total);
+            const float can = (p - 0.015f) * total, must = (p + 0.015f) * total;
             if (tid == 0) sh.found_bin = 0, sh.found = kValueBins - 1;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                if (at_high < can && can <= at_high + upper[i]) atomicMax(&sh.found_bin, first + i);
-                if (at_low < must && must <= at_low + lower[i]) atomicMin(&sh.found, first + i);
-                at_high += upper[i], at_low += lower[i];
+                if (at < can && can <= at + masses[i]) atomicMax(&sh.found_bin, first + i);
+                if (at < must && must <= at + masses[i]) atomicMin(&sh.found, first + i);
+                at += masses[i];
             }
             __syncthreads();
             const int open = sh.found_bin, close = sh.found;
             // tokens above the first bin and up to the last
-            const u64 counts_open = count_above(sh, first, seen - count, cnt, open);
-            const u64 counts_close = count_above(sh, first, seen - count, cnt, close + 1);
+            const u64 counts_open = count_above(first, seen - count, cnt, open);
+            const u64 counts_close = count_above(first, seen - count, cnt, close + 1);
             if (by_count) cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
-            const float edge = bin_top(open), above = nextafterf(edge, INFINITY);
+            const float bottom = fmaxf(bin_bottom(close), floor_v);
             const bool few = counts_close <= u64(kCap) && !by_count;
-            if (few) push_list(r, fmaxf(bin_bottom(close), floor_v));
-            const Pair* all = r.exchange(block_reduce(sh, kept_mass(r, above), add_pairs));
-            Pair sums{0, 0};
-            for (int q = 0; q < r.size; ++q) sums = add_pairs(sums, all[q]);
-            if (few) {
-                if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, sums.a);
+            if (few) push_list(r, bottom);
+            const auto exact = [&](float at) {
+                const Pair* all = r.exchange(block_reduce(kept_mass(r, at), add_pairs));
+                Pair sums{0, 0};
+                for (int q = 0; q < r.size; ++q) sums = add_pairs(sums, all[q]);
+                return sums;
+            };
+            const Pair mass = exact(bottom);
+            const u64 target = nucleus(mass.a, p);
+            const bool low_enough = mass.b >= target;
+            if (few && low_enough) {
+                if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, mass.a);
                 return true;
             }
-            cut_row<TY, true>(r, fmaxf(bin_bottom(close), floor_v), edge, sums.b, nucleus(sums.a, p), counts_close - counts_open);
+            const float edge = bin_top(open);
+            Row<TY> upper = r;  // what lies above the first bin
+            upper.keep_from(fmaxf(nextafterf(edge, INFINITY), r.edge));
+            const u64 base = [&] {
+                const Pair* all = r.exchange(block_reduce(kept_mass(upper, INFINITY), add_pairs));
+                u64 sum = 0;
+                for (int q = 0; q < r.size; ++q) sum += all[q].a;
+                return sum;
+            }();
+            const bool high_enough = base < target;
+            cut_row<TY, true>(r, low_enough ? bottom : r.weigh_from, high_enough ? edge : r.top, high_enough ? base : 0, target,
+                              low_enough && high_enough ? counts_close - counts_open : a.vocab);
         } else if (by_count) {
             cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
         }
-        draw_from_row(r, a, row, u);
+        draw_from_row(r, a, row, u, 0.f);
         return true;
     }
+}
+
+// The values of a counted vector above -128 that have no code.  1: NaN or
+// +inf; 2: 128 or more, 8: too many tiny ones.  (4: -128 or less but not -inf.)
+template <int TY>
+__device__ __noinline__ uint32_t note_others(const uint4 q, int part) {
+    constexpr int E = Elem<TY>::E;
+    Values& h = shared().values;
+    float x[E];
+    Elem<TY>::unpack(q, x);
+    uint32_t notes = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float size_of = fabsf(x[e]);
+        if (!(x[e] < INFINITY)) {
+            notes |= 1;
+        } else if (x[e] >= 128.f) {
+            notes |= 2;
+        } else if (size_of < 0x1p-10f) {
+            const uint32_t at = atomicAdd(&h.own[2 * kCodes], 1u);
+            if (TY == 0) {
+                if (at < uint32_t(kTinyCap)) h.tiny[at] = x[e], h.tiny_part[at] = uint8_t(part);
+                else notes |= 8;
+            }
+        }
+    }
+    return notes;
 }
 
 // One cluster per row.  The barrier of a cluster is the hardware's: all its
@@ -1081,9 +1269,7 @@ template <int TY>
 __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     using El = Elem<TY>;
     constexpr int E = El::E, kBatch = 4;
-    extern __shared__ uint4 dynamic[];
-    Shared& sh = *reinterpret_cast<Shared*>(dynamic);
-    uint4* const data = dynamic + sizeof(Shared) / 16;
+    Shared& sh = shared();
     auto cluster = cg::this_cluster();
     cluster.barrier_arrive();  // waited for before the first access to another CTA's shared memory
     const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -1097,13 +1283,14 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     const uint4* base = reinterpret_cast<const uint4*>(begin - lead * El::kBytes) + v0;
     const int i_first = v0 * E - lead;  // index of the first value
     const bool resident = a.resident;   // the logits stay in shared memory; else later passes find them in L2
+    const int head = i_first < 0 ? 0 : -1, tail = v0 + nvec == total_vecs && (lead + a.vocab) % E ? nvec - 1 : -1;
     uint4 q[kBatch];
     auto fetch = [&](int b) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const int v = b + j * kThreads + tid, i0 = i_first + v * E;
+            const int v = b + j * kThreads + tid;
             if (v < nvec)
-                q[j] = i0 >= 0 && i0 + E <= a.vocab ? __ldcg(base + v) : edge_vector<TY>(begin, i0, a.vocab);
+                q[j] = v != head && v != tail ? __ldcg(base + v) : edge_vector<TY>(begin, i_first + v * E, a.vocab);
         }
     };
     fetch(0);
@@ -1131,11 +1318,14 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         for (int i = tid; i < int(sizeof(h.all) / 16); i += kThreads) reinterpret_cast<uint4*>(h.all)[i] = make_uint4(0, 0, 0, 0);
     }
     const int frac = min(51, 62 - (32 - __clz((a.vocab - 1) | 1)));  // s
+    if (TY == 0 && a.part_rows)
+        for (int i = tid; i < kCodes; i += kThreads) vectors()[i] = make_uint4(0, 0, 0, 0);  // kParts / 2 * 2 * kCodes words
     if (tid < 256) sh.pow256[tid] = exp2(frac - tid * (1.0 / 256));
     if (tid == 0) sh.list.n = 0, sh.bound[0] = 0;
     __syncthreads();
     float top = -INFINITY;
-    uint32_t notes = 0;  // 1: NaN or +inf; 2: 128 or more, 4: -128 or less but not -inf, 8: too many tiny
+    bool strange = false, masked = false;
+    uint32_t notes = 0;  // of note_others
     for (int b = 0; b < nvec; b += kBatch * kThreads) {
         uint4 now[kBatch];
 #pragma unroll
@@ -1145,50 +1335,53 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         for (int j = 0; j < kBatch; ++j) {
             const int v = b + j * kThreads + tid;
             if (v >= nvec) break;
-            if (resident) data[v] = now[j];
+            if (resident) vectors()[v] = now[j];
             float x[E];
             El::unpack(now[j], x);
-            uint32_t others = 0;  // 1: a value without a code
             if (counting) {
+                const int part = TY == 0 && a.part_rows ? (b / kThreads + j) / a.part_rows : 0;
+                uint32_t* const counts = TY == 0 && a.part_rows ? parts() + (part >> 1) * 2 * kCodes : h.own;
+                const uint32_t one = 1u << (16 * (part & 1));
+                bool plain = true;  // every value has a code
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const uint32_t bits = __float_as_uint(x[e]) >> 16;
-                    const uint32_t code = (bits & 0x7fffu) - kFirstCode;
-                    if (code < uint32_t(kCodes)) atomicAdd(&h.own[code + (bits >> 15) * kCodes], 1u);
-                    others |= code >= uint32_t(kCodes);
+                    const uint32_t bits = __float_as_uint(x[e]), code = ((bits >> 16) & 0x7fffu) - kFirstCode;
+                    const bool coded = code < uint32_t(kCodes);
+                    if (coded) atomicAdd(&counts[code + (bits >> 31) * kCodes], one);
+                    plain = plain & coded;
+                }
+                if (!plain) {  // a mask's -inf, mostly
+                    bool others = false;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        others = others | !(fabsf(x[e]) >= 0x1p-10f & x[e] < 128.f);
+                        masked = masked | (x[e] <= -128.f & x[e] > -INFINITY);
+                    }
+                    if (others) notes |= note_others<TY>(now[j], part);
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) others |= !(x[e] < INFINITY);
+                for (int e = 0; e < E; ++e) strange = strange | !(x[e] < INFINITY);
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e) top = fmaxf(top, x[e]);
-            if (others) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float size_of = fabsf(x[e]);
-                    if (!(x[e] < INFINITY)) {
-                        notes |= 1;
-                    } else if (size_of >= 128.f) {
-                        if (size_of < INFINITY) notes |= x[e] > 0.f ? 2 : 4;
-                    } else if (counting && size_of < 0x1p-10f) {
-                        const uint32_t at = atomicAdd(&h.own[2 * kCodes], 1u);
-                        if (TY == 0) {
-                            if (at < uint32_t(kTinyCap)) h.tiny[at] = x[e];
-                            else notes |= 8;
-                        }
-                    }
-                }
-            }
+            top = fmaxf(top, El::largest(now[j]));
         }
     }
 
-    Row<TY> r{sh, resident ? data : nullptr, base, begin, a.vocab, nvec, i_first, rank, size, 0};
+    Row<TY> r{resident, head, tail, base, begin, a.vocab, nvec, i_first, rank, size, 0};
     auto join = [](Pair x, Pair y) { return Pair{as_bits(fmaxf(as_float(x.a), as_float(y.a))), x.b | y.b}; };
-    const Pair mine = block_reduce(sh, Pair{as_bits(top), notes}, join);
+    const Pair mine = block_reduce(Pair{as_bits(top), notes | uint32_t(strange) | uint32_t(masked) << 2}, join);
+    if (TY == 0 && a.part_rows)
+        for (int i = tid; i < 2 * kCodes; i += kThreads) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) c += part_count(i, part);
+            h.own[i] = c;
+        }
+    // Uncut at T = 1, the weights are those exponentials (fp16, fp32; the counts of bf16 give them anyhow).
+    const bool from_mass = TY != 0 && a.logprobs && T == 1.f && !cuts && min_p == 0.f && u != 0.f;
     // sum of exponentials for the log probability, against this CTA's largest logit; a bf16 row takes it from its counts
     Pair sums{0, 0};
-    if (TY != 0 && a.logprobs) {
+    if (TY != 0 && a.logprobs && !from_mass) {
         const float local = as_float(mine.a);
         float equal = 0.f, others = 0.f;
         r.each([&](float x, int) {
@@ -1196,7 +1389,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
             equal += x == local ? 1.f : 0.f;
             others += x == local ? 0.f : e;
         });
-        sums = block_reduce(sh, Pair{as_bits(equal), as_bits(others)}, add_floats);
+        sums = block_reduce(Pair{as_bits(equal), as_bits(others)}, add_floats);
     }
     cluster.barrier_wait();
     const uint32_t own_tiny = counting ? h.own[2 * kCodes] : 0;
@@ -1241,7 +1434,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
             equal += x == top ? 1.f : 0.f;
             others += x == top ? 0.f : e;
         });
-        const Pair own = block_reduce(sh, Pair{as_bits(equal), as_bits(others)}, add_floats);
+        const Pair own = block_reduce(Pair{as_bits(equal), as_bits(others)}, add_floats);
         if (tid < size) *cluster.map_shared_rank(&sh.part[rank], tid) = Pair{as_bits(top), own.a | own.b << 32};
         cluster.sync();
     }
@@ -1255,7 +1448,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
             if (x > El::kLowest) low = fminf(low, x);
         });
         auto least = [](Pair x, Pair y) { return Pair{as_bits(fminf(as_float(x.a), as_float(y.a))), 0}; };
-        all = r.exchange(block_reduce(sh, Pair{as_bits(low), 0}, least));
+        all = r.exchange(block_reduce(Pair{as_bits(low), 0}, least));
         for (int i = 0; i < size; ++i) low = fminf(low, as_float(all[i].a));
         if (double(top) - 746.0 * double(T) <= double(El::kLowest)) low = El::kLowest;
         const auto from = [&](double units) {
@@ -1265,14 +1458,14 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         if (by_mass) {
             const bool counted = r.count_mode;
             r.weigh(false, frac, T);  // the nucleus goes by mass for u = 0 too
-            all = r.exchange(block_reduce(sh, kept_mass(r, top), add_pairs));
+            all = r.exchange(block_reduce(kept_mass(r, top), add_pairs));
             u64 mass = 0;
             for (int i = 0; i < size; ++i) mass += all[i].a;
             cut_row<TY, true>(r, from(37.0), top, 0, nucleus(mass, p), a.vocab);
             r.weigh(counted, frac, T);
         }
     }
-    draw_from_row(r, a, row, u);
+    draw_from_row(r, a, row, u, from_mass ? 1.f / float(1ull << frac) : 0.f);
 }
 
 std::atomic<bool> g_attr[3][64];
@@ -1341,7 +1534,8 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(M) * unsigned(size));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(Shared) + (a.resident ? size_t(a.vecs) * 16 : 0);
+    a.part_rows = type == 0 && !a.resident && a.vecs >= kParts * kThreads ? ((a.vecs + kThreads - 1) / kThreads + kParts - 1) / kParts : 0;
+    cfg.dynamicSmemBytes = sizeof(Shared) + (a.resident ? size_t(a.vecs) * 16 : a.part_rows ? size_t(kCodes) * 16 : 0);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
