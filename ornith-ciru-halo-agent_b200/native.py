@@ -781,25 +781,13 @@ def w4_pack(codes, scales, zeros=None):
 
 def _launch_on(index, fn, *args):
     """fn(*args, current stream of device `index`) with that device current:
-    the caller's current device may be another one.  The raw stream query costs
-    a small part of torch.cuda.current_stream, which makes an object; calls of
-    this size are bound by the host."""
-    if index == torch.cuda.current_device():
+    the caller's current device may be another one.  The raw queries cost a
+    small part of torch.cuda's, which make objects; calls of this size are
+    bound by the host."""
+    if index == torch._C._cuda_getDevice():
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
-
-
-def _w4_bank_fits(tiles, scales, zeros, n, k, index):
-    """Whether (tiles, scales, zeros) is what w4_pack returns for [n, k] on that device."""
-    if scales.dim() != 3 or not scales.shape[1] or k % scales.shape[1] or scales.dtype not in _W4_TYPES:
-        return False
-    tile_shape, scale_shape, zero_shape = w4_pack_shapes(n, k, k // scales.shape[1])
-    return (tiles.shape == tile_shape and tiles.dtype is torch.uint32 and scales.shape == scale_shape
-            and tiles.get_device() == index and scales.get_device() == index and tiles.is_contiguous()
-            and scales.is_contiguous()
-            and (zeros is None or (zeros.shape == zero_shape and zeros.dtype is torch.uint8
-                                   and zeros.get_device() == index and zeros.is_contiguous())))
 
 
 def w4_launch(x, tiles, scales, zeros, out, flags, n, k):
@@ -808,23 +796,30 @@ def w4_launch(x, tiles, scales, zeros, out, flags, n, k):
     x may have rows further apart than k (a multiple of 8 values, rows on 16
     bytes).  flags receives the dense bits 4 (non-finite result) and 8
     (non-finite stored value)."""
-    index = x.get_device()
-    if (x.dim() != 2 or x.shape[1] != k or x.shape[0] > W4_ROWS or x.dtype not in _W4_TYPES or index < 0
-            or x.stride(1) != 1):
+    index, dtype, shape = x.get_device(), x.dtype, x.shape
+    if len(shape) != 2 or shape[1] != k or shape[0] > W4_ROWS or dtype not in _W4_TYPES or index < 0:
         raise ValueError(f'w4_launch takes CUDA bf16 or fp16 rows [M <= {W4_ROWS}, {k}]')
-    m, stride, at = x.shape[0], x.stride(0), x.data_ptr()
-    if at % 16 or (m > 1 and (stride < k or stride % 8)):
+    m, (stride, inner), at = shape[0], x.stride(), x.data_ptr()
+    if inner != 1 or at % 16 or (m > 1 and (stride < k or stride % 8)):
         raise ValueError('w4_launch takes rows that start on 16 bytes and do not overlap')
-    if (out.shape != (m, n) or (out.dtype is not x.dtype and out.dtype is not torch.float32)
+    out_dtype = out.dtype
+    if (out.shape != (m, n) or (out_dtype is not dtype and out_dtype is not torch.float32)
             or out.get_device() != index or not out.is_contiguous()):
         raise ValueError(f'w4_launch writes a contiguous [M, {n}] of the type of x or fp32 on the device of x')
-    if not _w4_bank_fits(tiles, scales, zeros, n, k, index):
+    bank = scales.shape
+    group = k // bank[1] if len(bank) == 3 and bank[1] else 0
+    tile_shape, scale_shape, zero_shape = w4_pack_shapes(n, k, group)
+    if (bank != scale_shape or tiles.shape != tile_shape or tiles.dtype is not torch.uint32
+            or scales.dtype not in _W4_TYPES or tiles.get_device() != index or scales.get_device() != index
+            or not tiles.is_contiguous() or not scales.is_contiguous()
+            or (zeros is not None and (zeros.shape != zero_shape or zeros.dtype is not torch.uint8
+                                       or zeros.get_device() != index or not zeros.is_contiguous()))):
         raise ValueError(f'w4_launch takes tiles, scales and zero points as w4_pack returns them for [{n}, {k}]')
     _check_flags(flags, index)
-    check(_launch_on(index, lib().ornith_moe_b200_w4_launch, at, stride, _TYPES[x.dtype], tiles.data_ptr(),
-                     scales.data_ptr(), _TYPES[scales.dtype], None if zeros is None else zeros.data_ptr(),
-                     out.data_ptr(), _TYPES[out.dtype], flags.data_ptr(), m, n, k, k // scales.shape[1]),
-          'W4 product')
+    status = _launch_on(index, lib().ornith_moe_b200_w4_launch, at, stride, _TYPES[dtype], tiles.data_ptr(),
+                        scales.data_ptr(), _TYPES[scales.dtype], None if zeros is None else zeros.data_ptr(),
+                        out.data_ptr(), _TYPES[out_dtype], flags.data_ptr(), m, n, k, group)
+    check(status, 'W4 product')
 
 
 def _check_flags(flags, index):
@@ -870,33 +865,33 @@ def sample_launch(logits, temperature, top_k, top_p, min_p, uniform, tokens, log
     raises a bit of flags: 1 NaN or +inf among its logits, 2 a parameter out of
     range (temperature outside [0, 1e30], negative top_p, min_p outside [0, 1],
     uniform outside [0, 1), any NaN), 4 every logit -inf."""
-    index = logits.get_device()
-    if (logits.dim() != 2 or logits.dtype not in _TYPES or index < 0 or not 0 < logits.shape[1] <= SAMPLE_MAX_VOCAB
-            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+    index, shape = logits.get_device(), logits.shape
+    if (len(shape) != 2 or logits.dtype not in _TYPES or index < 0 or not 0 < shape[1] <= SAMPLE_MAX_VOCAB
+            or (shape[1] > 1 and logits.stride(1) != 1)):
         raise ValueError(f'sample_launch takes CUDA bf16, fp16 or fp32 logits [M, V <= {SAMPLE_MAX_VOCAB}] with '
                          'neighbouring values')
-    m, vocab = logits.shape
+    m, vocab = shape
     stride = logits.stride(0) if m > 1 else vocab
     if stride < vocab:
         raise ValueError('sample_launch takes rows that do not overlap')
-    rows = [_row_pointer(t, name, dtype, m, index) for t, name, dtype in (
-        (temperature, 'temperature', torch.float32), (top_k, 'top_k', torch.int32), (top_p, 'top_p', torch.float32),
-        (min_p, 'min_p', torch.float32), (uniform, 'uniform', torch.float32), (tokens, 'tokens', torch.int32),
-        (logprobs, 'logprobs', torch.float32))]
     if uniform is None or tokens is None:
         raise ValueError('sample_launch needs uniform and tokens')
+    fp32, int32, rows = torch.float32, torch.int32, (m,)
+    at = [_row_pointer(temperature, 'temperature', fp32, rows, index), _row_pointer(top_k, 'top_k', int32, rows, index),
+          _row_pointer(top_p, 'top_p', fp32, rows, index), _row_pointer(min_p, 'min_p', fp32, rows, index),
+          _row_pointer(uniform, 'uniform', fp32, rows, index), _row_pointer(tokens, 'tokens', int32, rows, index),
+          _row_pointer(logprobs, 'logprobs', fp32, rows, index)]
     _check_flags(flags, index)
     check(_launch_on(index, lib().ornith_moe_b200_sample_launch, logits.data_ptr(), stride, _TYPES[logits.dtype],
-                     *rows, flags.data_ptr(), m, vocab), 'sampling')
+                     *at, flags.data_ptr(), m, vocab), 'sampling')
 
 
 def _row_pointer(t, name, dtype, rows, index):
     """The address of a row parameter, None for one that is not given."""
     if t is None:
         return None
-    if (t.dtype is not dtype or t.dim() != 1 or t.shape[0] != rows or t.get_device() != index
-            or not t.is_contiguous()):
-        raise ValueError(f'sample_launch takes {name} as a contiguous {dtype} [{rows}] on the device of the logits')
+    if t.dtype is not dtype or t.shape != rows or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f'sample_launch takes {name} as a contiguous {dtype} {list(rows)} on the device of the logits')
     return t.data_ptr()
 
 
