@@ -1235,6 +1235,14 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
     }
 }
 
+// *shared += v where `in`, without a branch: eight of them in a row would each
+// part and join the warp again.
+__device__ __forceinline__ void add_where(bool in, uint32_t shared_address, uint32_t v) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %0, 0; @p red.shared.add.u32 [%1], %2; }" ::"r"(uint32_t(in)),
+                 "r"(shared_address), "r"(v)
+                 : "memory");
+}
+
 // The values of a counted vector above -128 that have no code.  1: NaN or
 // +inf; 2: 128 or more, 8: too many tiny ones.  (4: -128 or less but not -inf.)
 template <int TY>
@@ -1340,14 +1348,14 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
             El::unpack(now[j], x);
             if (counting) {
                 const int part = TY == 0 && a.part_rows ? (b / kThreads + j) / a.part_rows : 0;
-                uint32_t* const counts = TY == 0 && a.part_rows ? parts() + (part >> 1) * 2 * kCodes : h.own;
-                const uint32_t one = 1u << (16 * (part & 1));
+                const uint32_t* const counts = TY == 0 && a.part_rows ? parts() + (part >> 1) * 2 * kCodes : h.own;
+                const uint32_t counts_at = uint32_t(__cvta_generic_to_shared(counts)), one = 1u << (16 * (part & 1));
                 bool plain = true;  // every value has a code
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const uint32_t bits = __float_as_uint(x[e]), code = ((bits >> 16) & 0x7fffu) - kFirstCode;
                     const bool coded = code < uint32_t(kCodes);
-                    if (coded) atomicAdd(&counts[code + (bits >> 31) * kCodes], one);
+                    add_where(coded, counts_at + 4 * (code + (bits >> 31) * kCodes), one);
                     plain = plain & coded;
                 }
                 if (!plain) {  // a mask's -inf, mostly
