@@ -489,9 +489,9 @@ ORNITH_MOE_B200_EXPORT int ornith_head_i8_tile_shortlist(void);
  * (value 8j + d of a row in bits 4d of its word j), scales 16-bit [N][K/group],
  * zeros uint8 [N][K/group] in 0..15 (only the low four bits are used) or null for 8 ->
  * tiles UINT32[ceil(N/16)][ceil(K/64)][32][4], tile_scales
- * UINT32[ceil(N/16)][K/group][8], tile_zeros uint8 [ceil(N/16)][K/group][8]
+ * UINT32[ceil(N/16)][K/group][8], tile_zeros uint8 [ceil(N/16)][K/group][16]
  * (null iff zeros is).  Buffers must not overlap.  Alignment: tiles 16 B, codes
- * and tile_scales 4 B, scales 2 B. */
+ * and tile_scales 4 B, scales and tile_zeros 2 B. */
 ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_w4_pack(
     const void* codes, const void* scales_16, const void* zeros_u8, void* tiles, void* tile_scales,
     void* tile_zeros, int N, int K, int group, cudaStream_t stream);
@@ -500,7 +500,7 @@ ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_w4_pack(
  * unused for one row) -> out [M][N] of x_type or fp32.  scale_type is the type
  * of the packed scales, tile_zeros null for zero points of 8.  M == 0 returns
  * success without touching a pointer.  No workspace.  Alignment: x and tiles
- * 16 B, tile_scales and flags 4 B, out its type's; out and flags overlap
+ * 16 B, tile_scales and flags 4 B, tile_zeros 2 B, out its type's; out and flags overlap
  * nothing. */
 ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_w4_launch(
     const void* x, int64_t x_stride, int x_type, const void* tiles, const void* tile_scales, int scale_type,

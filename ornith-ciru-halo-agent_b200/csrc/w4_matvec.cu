@@ -38,7 +38,7 @@ void count_launches(int n);
 
 namespace w4 {
 
-constexpr int kMaxM = 16, kWarps = 8, kMaxK = 16384, kMaxN = 1 << 22, kSms = 148;
+constexpr int kMaxM = 16, kMaxK = 16384, kMaxN = 1 << 22, kSms = 148;
 constexpr uint32_t kFlagProjection = 4, kFlagStored = 8;  // the dense library's bits
 
 bool shape_ok(int N, int K, int group) {
@@ -81,9 +81,9 @@ __global__ __launch_bounds__(256) void w4_pack_codes_kernel(const uint32_t* code
 }
 
 // Scales 16-bit [N][K/G] -> [row tile][group][r] pairs (row r, row r + 8);
-// zero points u8 likewise, the pair in one byte.
+// zero points u8 likewise, a pair in two bytes.
 __global__ __launch_bounds__(256) void w4_pack_meta_kernel(const uint16_t* scales, const uint8_t* zeros,
-                                                           uint32_t* tile_scales, uint8_t* tile_zeros, int N,
+                                                           uint32_t* tile_scales, uint16_t* tile_zeros, int N,
                                                            int groups, size_t pairs) {
     const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= pairs) return;
@@ -96,10 +96,10 @@ __global__ __launch_bounds__(256) void w4_pack_meta_kernel(const uint16_t* scale
         if (row + 8 * h < N) {
             const size_t at = size_t(row + 8 * h) * groups + g;
             s |= uint32_t(scales[at]) << (16 * h);
-            if (zeros) z |= (zeros[at] & 15u) << (4 * h);
+            if (zeros) z |= (zeros[at] & 15u) << (8 * h);
         }
     tile_scales[i] = s;
-    if (zeros) tile_zeros[i] = uint8_t(z);
+    if (zeros) tile_zeros[i] = uint16_t(z);
 }
 
 // ---------------------------------------------------------------------------
@@ -111,11 +111,11 @@ struct Args {
     int64_t x_stride;  // values between rows of x
     const uint4* tiles;
     const uint32_t* scales;
-    const uint8_t* zeros;
+    const uint16_t* zeros;  // pairs of bytes
     void* out;
     uint32_t* flags;
     // per_warp: chunks of one warp, a multiple of a group's; split: warps that share a row tile
-    int M, N, K, chunks, groups, per_warp, split, out_f32, scale_f16;
+    int M, N, K, chunks, groups, per_warp, split, out_f32;
 };
 
 // A fragment register as the codes' exponent trick leaves it, 128 + c (bf16) or
@@ -125,7 +125,11 @@ template <bool F16>
 struct Num {
     static constexpr uint32_t kMagic = F16 ? 0x64006400u : 0x43004300u;
     static constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
-    static __device__ __forceinline__ uint32_t bias(uint32_t z) { return (z * 0x10001u) | kMagic | 0x80008000u; }
+    static constexpr uint32_t kBias = F16 ? 0xe4u : 0xc3u;  // high byte of -(1024 + z), -(128 + z)
+    // -(1024 + z) or -(128 + z) in both halves, z the low (half 0) or high byte of a pair
+    static __device__ __forceinline__ uint32_t bias(uint32_t pair, int half) {
+        return __byte_perm(pair, kBias, half ? 0x4141 : 0x4040);
+    }
     // (v & mask) | magic in one instruction
     static __device__ __forceinline__ uint32_t nibbles(uint32_t v) {
         uint32_t d;
@@ -158,8 +162,9 @@ struct Num {
     }
 };
 
-__device__ __forceinline__ float scale_value(uint32_t bits16, int f16) {
-    return f16 ? __half2float(__ushort_as_half(uint16_t(bits16))) : __uint_as_float(bits16 << 16);
+template <bool F16>
+__device__ __forceinline__ float scale_value(uint32_t bits16) {
+    return F16 ? __half2float(__ushort_as_half(uint16_t(bits16))) : __uint_as_float(bits16 << 16);
 }
 
 // Streamed once: do not keep the codes in L1.
@@ -171,22 +176,29 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
     return v;
 }
 
-// kWarps warps; `split` warps (a power of two up to kWarps) share TILES row
-// tiles, each with a range of their chunks, and join their sums through shared
-// memory.  MT: tiles of 8 activation rows.  Rows past M repeat the last one:
+// `split` warps of a CTA (a power of two) share TILES row tiles, each with a
+// range of their chunks, and join their sums through shared memory.  MT: tiles
+// of 8 activation rows; S16: fp16 scales.  Rows past M repeat the last one:
 // columns of the product are independent and theirs are not stored.
-template <bool F16, int MT, bool ZP, int GROUP, int TILES>
-__global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
+//
+// CTAs of four warps and at least 20 warps on an SM where a warp takes two row
+// tiles: 68 us for 8 rows of the head, against 78 with eight warps to a CTA
+// and 94 with registers cut for 28 warps.
+template <int TILES>
+constexpr int kWarps = TILES == 2 ? 4 : 8;
+template <bool F16, bool S16, int MT, bool ZP, int GROUP, int TILES>
+__global__ __launch_bounds__(kWarps<TILES> * 32, TILES == 2 ? 5 : 3) void w4_matvec_kernel(const Args a) {
+    constexpr int kThreads = kWarps<TILES> * 32;
     constexpr int kRuns = GROUP == 32 ? 2 : 1;             // groups in a chunk
     constexpr int kSpan = GROUP < 64 ? 1 : GROUP / 64;     // chunks of a group
     // Chunks in flight.  Registers, and with them warps, count for more than depth where a warp
     // holds two tiles of rows or of N: 2 against 4 took 76 us against 85 for 8 rows of the head.
     constexpr int kAhead = (MT * TILES > 1 || GROUP == 32) && kSpan <= 2 ? 2 : 4;
     constexpr int kMeta = kAhead / kSpan;                  // scales in flight, per run
-    __shared__ float joined[kWarps][TILES][16][8 * MT + 1];
+    __shared__ float joined[kWarps<TILES>][TILES][16][8 * MT + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
     const int part = warp & (a.split - 1);
-    const int per_cta = kWarps / a.split;  // warps of different row tiles
+    const int per_cta = kWarps<TILES> / a.split;  // warps of different row tiles
     const int row_tile = (blockIdx.x * per_cta + warp / a.split) * TILES, row_tiles = (a.N + 15) / 16;
     const int first = part * a.per_warp;
     int left = row_tile < row_tiles ? min(a.per_warp, a.chunks - first) : 0;
@@ -201,7 +213,7 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
     if (left > 0) {
         const uint4* tile[TILES];
         const uint32_t* scale[TILES];
-        const uint8_t* zero[TILES];
+        const uint16_t* zero[TILES];
 #pragma unroll
         for (int q = 0; q < TILES; ++q) {
             const int of = min(row_tile + q, row_tiles - 1);  // an odd last tile is computed twice, stored once
@@ -258,8 +270,8 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
 #pragma unroll
                     for (int h = 0; h < kRuns; ++h) {
                         s2[q][h] = sc[q][d / kSpan][h];
-                        const uint32_t z = ZP ? zp[q][d / kSpan][h] : 0x88u;
-                        bias[q][h][0] = Num<F16>::bias(z & 15u), bias[q][h][1] = Num<F16>::bias(z >> 4);
+                        const uint32_t z = ZP ? zp[q][d / kSpan][h] : 0x808u;
+                        bias[q][h][0] = Num<F16>::bias(z, 0), bias[q][h][1] = Num<F16>::bias(z, 1);
                     }
                 }
                 // the group's scale is still needed by its later chunks: fetch after its last
@@ -290,8 +302,8 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
                     if (kRuns == 2 || (h == 1 && d % kSpan == kSpan - 1)) {
 #pragma unroll
                         for (int q = 0; q < TILES; ++q) {
-                            const float lo = scale_value(s2[q][g] & 0xffffu, a.scale_f16);
-                            const float hi = scale_value(s2[q][g] >> 16, a.scale_f16);
+                            const float lo = scale_value<S16>(s2[q][g] & 0xffffu);
+                            const float hi = scale_value<S16>(s2[q][g] >> 16);
 #pragma unroll
                             for (int i = 0; i < MT; ++i) {
                                 acc[q][i][0] = __fmaf_rn(lo, run[q][i][0], acc[q][i][0]);
@@ -323,7 +335,7 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
     __syncthreads();
     uint32_t fault = 0;
     const int rows = 16 * TILES * per_cta;  // rows of N of this CTA
-    for (int i = threadIdx.x; i < rows * a.M; i += kWarps * 32) {
+    for (int i = threadIdx.x; i < rows * a.M; i += kThreads) {
         const int m = i / rows, row = i % rows, n = blockIdx.x * rows + row;
         if (n >= a.N) continue;
         float v = 0.f;
@@ -346,13 +358,13 @@ __global__ __launch_bounds__(kWarps * 32) void w4_matvec_kernel(const Args a) {
     if (fault) atomicOr(a.flags, fault);
 }
 
-template <bool F16, int MT, bool ZP, int TILES>
+template <bool F16, bool S16, int MT, bool ZP, int TILES>
 void launch(const Args& a, int group, int blocks, cudaStream_t stream) {
-    auto* kernel = group == 32    ? w4_matvec_kernel<F16, MT, ZP, 32, TILES>
-                   : group == 64  ? w4_matvec_kernel<F16, MT, ZP, 64, TILES>
-                   : group == 128 ? w4_matvec_kernel<F16, MT, ZP, 128, TILES>
-                                  : w4_matvec_kernel<F16, MT, ZP, 256, TILES>;
-    kernel<<<blocks, kWarps * 32, 0, stream>>>(a);
+    auto* kernel = group == 32    ? w4_matvec_kernel<F16, S16, MT, ZP, 32, TILES>
+                   : group == 64  ? w4_matvec_kernel<F16, S16, MT, ZP, 64, TILES>
+                   : group == 128 ? w4_matvec_kernel<F16, S16, MT, ZP, 128, TILES>
+                                  : w4_matvec_kernel<F16, S16, MT, ZP, 256, TILES>;
+    kernel<<<blocks, kWarps<TILES> * 32, 0, stream>>>(a);
 }
 
 }  // namespace w4
@@ -373,8 +385,8 @@ extern "C" cudaError_t ornith_moe_b200_w4_pack(const void* codes, const void* sc
     if (!buffers_ok(ptr, size, align, 2, 4)) return cudaErrorInvalidValue;
     if (zeros) {
         const void* const zptr[6] = {codes, scales, zeros, tiles, tile_scales, tile_zeros};
-        const size_t zsize[6] = {size[0], size[1], size_t(N) * groups, size[2], size[3], pairs};
-        const uintptr_t zalign[6] = {4, 2, 1, 16, 4, 1};
+        const size_t zsize[6] = {size[0], size[1], size_t(N) * groups, size[2], size[3], pairs * 2};
+        const uintptr_t zalign[6] = {4, 2, 1, 16, 4, 2};
         if (!buffers_ok(zptr, zsize, zalign, 3)) return cudaErrorInvalidValue;
     }
     count_launches(2);
@@ -384,7 +396,7 @@ extern "C" cudaError_t ornith_moe_b200_w4_pack(const void* codes, const void* sc
     if (st != cudaSuccess) return st;
     w4_pack_meta_kernel<<<unsigned((pairs + 255) / 256), 256, 0, stream>>>(
         static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), static_cast<uint32_t*>(tile_scales),
-        static_cast<uint8_t*>(tile_zeros), N, groups, pairs);
+        static_cast<uint16_t*>(tile_zeros), N, groups, pairs);
     return cudaGetLastError();
 }
 
@@ -406,33 +418,36 @@ extern "C" cudaError_t ornith_moe_b200_w4_launch(const void* x, int64_t x_stride
     const size_t pairs = size_t(row_tiles(N)) * groups * 8;
     const void* const ptr[6] = {x, tiles, tile_scales, tile_zeros, out, flags};
     const size_t size[6] = {(size_t(M - 1) * size_t(x_stride) + size_t(K)) * 2, size_t(row_tiles(N)) * k_chunks(K) * 512,
-                            pairs * 4, pairs, size_t(M) * N * (out_type == 2 ? 4 : 2), 4};
-    const uintptr_t align[6] = {16, 16, 4, 1, uintptr_t(out_type == 2 ? 4 : 2), 4};
+                            pairs * 4, pairs * 2, size_t(M) * N * (out_type == 2 ? 4 : 2), 4};
+    const uintptr_t align[6] = {16, 16, 4, 2, uintptr_t(out_type == 2 ? 4 : 2), 4};
     if (!buffers_ok(ptr, size, align, 4, 3)) return cudaErrorInvalidValue;  // zero points may be null
     NvtxRange range("ornith.w4");
     Args a{};
     a.x = x, a.x_stride = x_stride;
     a.tiles = static_cast<const uint4*>(tiles);
     a.scales = static_cast<const uint32_t*>(tile_scales);
-    a.zeros = static_cast<const uint8_t*>(tile_zeros);
+    a.zeros = static_cast<const uint16_t*>(tile_zeros);
     a.out = out, a.flags = static_cast<uint32_t*>(flags);
     a.M = M, a.N = N, a.K = K, a.chunks = k_chunks(K), a.groups = groups;
-    a.out_f32 = out_type == 2, a.scale_f16 = scale_type;
+    a.out_f32 = out_type == 2;
     const int span = group < 64 ? 1 : group / 64, units = (a.chunks + span - 1) / span;
     // Row tiles of a warp: two share its activations where that leaves 16 warps on each SM.
     const int tiles_each = row_tiles(N) >= 2 * kSms * 16 ? 2 : 1, sets = (row_tiles(N) + tiles_each - 1) / tiles_each;
+    const int warps = tiles_each == 2 ? kWarps<2> : kWarps<1>;
     // Warps that share row tiles: as few as keep 16 warps on each SM.
     a.split = 1;
-    while (a.split < kWarps && a.split < units && sets * a.split < kSms * 16) a.split *= 2;
+    while (a.split < warps && a.split < units && sets * a.split < kSms * 16) a.split *= 2;
     a.per_warp = (units + a.split - 1) / a.split * span;
-    const int per_cta = kWarps / a.split, blocks = (sets + per_cta - 1) / per_cta;
+    const int per_cta = warps / a.split, blocks = (sets + per_cta - 1) / per_cta;
     count_launches(1);
     using Launch = void (*)(const Args&, int, int, cudaStream_t);
-#define ORNITH_W4(F16, MT) \
-    {{launch<F16, MT, false, 1>, launch<F16, MT, false, 2>}, {launch<F16, MT, true, 1>, launch<F16, MT, true, 2>}}
-    static constexpr Launch table[2][2][2][2] = {{ORNITH_W4(false, 1), ORNITH_W4(false, 2)},
-                                                 {ORNITH_W4(true, 1), ORNITH_W4(true, 2)}};
+#define ORNITH_W4(F16, S16, MT)                                              \
+    {{launch<F16, S16, MT, false, 1>, launch<F16, S16, MT, false, 2>}, \
+     {launch<F16, S16, MT, true, 1>, launch<F16, S16, MT, true, 2>}}
+    static constexpr Launch table[2][2][2][2][2] = {
+        {{ORNITH_W4(false, false, 1), ORNITH_W4(false, false, 2)}, {ORNITH_W4(false, true, 1), ORNITH_W4(false, true, 2)}},
+        {{ORNITH_W4(true, false, 1), ORNITH_W4(true, false, 2)}, {ORNITH_W4(true, true, 1), ORNITH_W4(true, true, 2)}}};
 #undef ORNITH_W4
-    table[x_type][M > 8][tile_zeros != nullptr][tiles_each - 1](a, group, blocks, stream);
+    table[x_type][scale_type][M > 8][tile_zeros != nullptr][tiles_each - 1](a, group, blocks, stream);
     return cudaGetLastError();
 }

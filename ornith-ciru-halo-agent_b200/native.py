@@ -746,7 +746,7 @@ def w4_pack_shapes(n, k, group):
         raise ValueError(f'a 4-bit weight has groups of 32, 64, 128 or 256, K a multiple of the group up to '
                          f'{W4_MAX_K} and N up to {W4_MAX_N}; got N {n}, K {k}, group {group}')
     row_tiles = -(-n // 16)
-    return (row_tiles, -(-k // 64), 32, 4), (row_tiles, k // group, 16), (row_tiles, k // group, 8)
+    return (row_tiles, -(-k // 64), 32, 4), (row_tiles, k // group, 16), (row_tiles, k // group, 16)
 
 
 def w4_pack(codes, scales, zeros=None):

@@ -26,7 +26,7 @@ def test_shapes(native, n, k, group, ok):
     if ok:
         tile_shape, scale_shape, zero_shape = native.w4_pack_shapes(n, k, group)
         assert tile_shape[0] * 16 >= n and tile_shape[1] * 64 >= k and scale_shape[1] * group == k
-        assert zero_shape[2] * 2 == scale_shape[2] == 16
+        assert zero_shape[2] == scale_shape[2] == 16
     else:
         with pytest.raises(ValueError):
             native.w4_pack_shapes(n, k, group)
