@@ -52,7 +52,8 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kMaxVocab = 1 << 19, kSms = 148;
-constexpr int kBins = 1024, kCap = 256, kAhead = 4;  // kAhead: vectors of a thread in flight
+constexpr int kBins = 1024, kCap = 256, kList = 2 * kThreads;  // bins of a search, candidates it ranks, tokens of a list
+constexpr int kAhead = 4;                                      // vectors of a thread in flight
 constexpr int kMaxVecs = 60 * kThreads, kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
 // 16-byte vectors of a CTA: at most, and kept on chip by one or two CTAs of an SM
 constexpr int kParts = 4;  // of a bf16 CTA's logits that do not stay on chip, counted apart in 16 bits: 15 * kThreads * 8 < 2^16
@@ -158,8 +159,17 @@ constexpr uint32_t kFirstCode = (134 - kOctaves) << 7;         // of 2^-10
 // Bins by value, largest first: the tiny between, the negative from a multiple of 4 on (three bins stay empty).
 constexpr int kTinyBin = kCodes, kNegative = kCodes + 4, kValueBins = kNegative + kCodes;
 constexpr int kPerThread = (kValueBins + kThreads - 1) / kThreads, kTinyCap = 256;
+// The tokens that can be kept, where they are few: pushed to the first CTA.
+struct List {
+    u64 weight[kList];                             // by rank
+    float v[kList];
+    int i[kList];
+};
 struct Values {
-    alignas(16) uint32_t own[2 * kCodes + 4];      // by code: positive, negative, tiny
+    union {
+        alignas(16) uint32_t own[2 * kCodes + 4];  // by code: positive, negative, tiny
+        List list;                                 // once the counts are merged
+    };
     alignas(16) uint32_t all[kPerThread * kThreads];  // the row's, by value
     float tiny[kTinyCap];                          // this CTA's tiny logits (bf16 rows)
     uint8_t tiny_part[kTinyCap];                   // and where they lie
@@ -189,20 +199,14 @@ __device__ __forceinline__ float bin_bottom(int bin) {
     return bin < kTinyBin ? near_edge(bin) : far_edge(bin);
 }
 
-// The tokens that can be kept, where they are few: pushed to the first CTA.
-struct List {
-    u64 weight[kCap];                    // by rank
-    float v[kCap], ranked_v[kCap];
-    int i[kCap], ranked_i[kCap];
-    uint32_t n;
-};
-
 struct alignas(16) Shared {
     union {
         Search search;
         Values values;
     };
-    List list;
+    float ordered_v[kList];              // the list by bin
+    int ordered_i[kList];
+    uint32_t listed;
     double pow256[256];                  // 2^(s - j/256)
     Pair slot[2][kMaxCluster];           // pushed by every CTA of the cluster in turn
     u64 slab[kSlabs];                    // kept mass of each slab, in index order
@@ -841,12 +845,13 @@ __device__ Partition counted_partition(const Row<0>& r) {
     return Partition{as_float(sums.a), as_float(sums.b)};
 }
 
-// Pushes the tokens at `bottom` or above (kCap at most) to the cluster's first
+// Pushes the tokens at `bottom` or above (kList at most) to the cluster's first
 // CTA.  The caller synchronises the cluster next.
 template <int TY>
 __device__ void push_list(const Row<TY>& r, float bottom) {
     auto cluster = cg::this_cluster();
-    List& l = *cluster.map_shared_rank(&shared().list, 0);
+    List& l = *cluster.map_shared_rank(&shared().values.list, 0);
+    uint32_t* const listed = cluster.map_shared_rank(&shared().listed, 0);
     r.each_vector([&](int v, const uint4& q) {
         if (Elem<TY>::largest(q) < bottom) return;
         float x[Elem<TY>::E];
@@ -854,10 +859,67 @@ __device__ void push_list(const Row<TY>& r, float bottom) {
 #pragma unroll
         for (int e = 0; e < Elem<TY>::E; ++e)
             if (x[e] >= bottom) {
-                const uint32_t at = atomicAdd(&l.n, 1u);
-                if (at < uint32_t(kCap)) l.v[at] = x[e], l.i[at] = r.first + v * Elem<TY>::E + e;
+                const uint32_t at = atomicAdd(listed, 1u);
+                if (at < uint32_t(kList)) l.v[at] = x[e], l.i[at] = r.first + v * Elem<TY>::E + e;
             }
     });
+}
+
+// Ranks the list by (value, index) into itself, with the weights of the first
+// `limit`.  Few tokens are compared with each other; more are first put in
+// order of their bins, whose counts say where each bin starts.
+template <int TY>
+__device__ __forceinline__ void rank_list(const Row<TY>& r, int n, u64 limit) {
+    Shared& sh = shared();
+    List& l = sh.values.list;
+    const int tid = threadIdx.x;
+    const auto before = [](float x, int i, float y, int j) { return x > y || (x == y && i < j); };
+    const auto put = [&](int rank, float x, int index) {
+        l.weight[rank] = u64(rank) < limit ? r.weight(x) : 0, l.v[rank] = x, l.i[rank] = index;
+    };
+    if (n <= kThreads / 2) {
+        const int e = tid >> 1, half = tid & 1;  // two threads a token
+        int rank = 0, index = 0;
+        float x = 0.f;
+        if (e < n) {
+            x = l.v[e], index = l.i[e];
+            for (int j = half; j < n; j += 2) rank += before(l.v[j], l.i[j], x, index);
+        }
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        __syncthreads();
+        if (e < n && half == 0) put(rank, x, index);
+        __syncthreads();
+        return;
+    }
+    uint32_t* const start = sh.values.all;
+    const auto bin_of = [](float x) {
+        const uint32_t bits = __float_as_uint(x), code = ((bits >> 16) & 0x7fffu) - kFirstCode;
+        return int(code < uint32_t(kCodes) ? (bits >> 31 ? kNegative + code : kCodes - 1 - code) : uint32_t(kTinyBin));
+    };
+    uint32_t count = 0;
+    for (int i = 0; i < kPerThread; ++i) count += start[tid * kPerThread + i];
+    uint32_t at = uint32_t(block_exclusive(count));
+    for (int i = 0; i < kPerThread; ++i) {
+        const uint32_t c = start[tid * kPerThread + i];
+        start[tid * kPerThread + i] = at, at += c;
+    }
+    __syncthreads();
+    for (int e = tid; e < n; e += kThreads) {
+        const float x = l.v[e];
+        const uint32_t place = min(atomicAdd(&start[bin_of(x)], 1u), uint32_t(kList - 1));
+        sh.ordered_v[place] = x, sh.ordered_i[place] = l.i[e];
+    }
+    __syncthreads();
+    // start is now each listed bin's end; all the bins before one are listed whole
+    for (int e = tid; e < n; e += kThreads) {
+        const float x = sh.ordered_v[e];
+        const int index = sh.ordered_i[e], bin = bin_of(x), to = min(int(start[bin]), n);
+        int rank = bin ? min(int(start[bin - 1]), n) : 0;
+        const int from = rank;
+        for (int j = from; j < to; ++j) rank += before(sh.ordered_v[j], sh.ordered_i[j], x, index);
+        put(rank, x, index);
+    }
+    __syncthreads();
 }
 
 // The first CTA ranks its list, applies top-k (`limit`) and top-p and draws.
@@ -865,8 +927,8 @@ __device__ void push_list(const Row<TY>& r, float bottom) {
 template <int TY>
 __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 limit, float p, float u, u64 whole) {
     Shared& sh = shared();
-    List& l = sh.list;
-    const int tid = threadIdx.x, n = min(int(l.n), kCap);
+    List& l = sh.values.list;
+    const int tid = threadIdx.x, n = min(int(sh.listed), kList);
     Partition z{1.f, 0.f};
     if (a.logprobs) {
         if constexpr (TY == 0)
@@ -874,43 +936,62 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
         else
             z = joined_partition(r);
     }
-    // two threads a token; the order of the list varies, the ranks do not
-    const int e = tid >> 1, half = tid & 1;
-    int rank = 0;
-    float x = 0.f;
-    int index = 0;
-    if (e < n) {
-        x = l.v[e], index = l.i[e];
-        for (int j = half; j < n; j += 2) rank += l.v[j] > x || (l.v[j] == x && l.i[j] < index);
-    }
-    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-    if (e < n && half == 0) l.weight[rank] = u64(rank) < limit ? r.weight(x) : 0, l.ranked_v[rank] = x, l.ranked_i[rank] = index;
+    rank_list(r, n, limit);
+    // two ranks a thread
     if (tid == 0) sh.found_bin = int(min(u64(n), limit)) - 1;
-    __syncthreads();
-    u64 w = tid < n ? l.weight[tid] : 0;
+    const u64 w0 = 2 * tid < n ? l.weight[2 * tid] : 0, w1 = 2 * tid + 1 < n ? l.weight[2 * tid + 1] : 0;
+    const u64 before = block_exclusive(w0 + w1);
     if (p < 1.f) {
-        const u64 before = block_exclusive(w);
-        if (tid == kThreads - 1) sh.bound[0] = before + w;
+        if (tid == kThreads - 1) sh.bound[0] = before + w0 + w1;
         __syncthreads();
         const u64 target = nucleus(whole ? whole : sh.bound[0], p);
-        if (before < target && target <= before + w) sh.found_bin = tid;
-        __syncthreads();
+        if (before < target && target <= before + w0) sh.found_bin = 2 * tid;
+        if (before + w0 < target && target <= before + w0 + w1) sh.found_bin = 2 * tid + 1;
     }
+    __syncthreads();
     const int keep = sh.found_bin + 1;
-    const u64 mass = block_reduce(Pair{tid < keep ? w : 0, 0}, add_pairs).a;
+    const u64 mass = block_reduce(Pair{(2 * tid < keep ? w0 : 0) + (2 * tid + 1 < keep ? w1 : 0), 0}, add_pairs).a;
     const u64 target = drawn(mass, u);
-    // mass up to each kept token in index order
-    w = 0;
-    u64 upto = 0;
-    if (e < keep) {
-        index = l.ranked_i[e], w = l.weight[e];
-        for (int j = half; j < keep; j += 2)
-            if (l.ranked_i[j] <= index) upto += l.weight[j];
+    const auto answer = [&](int rank) {
+        a.tokens[row] = l.i[rank];
+        if (a.logprobs) a.logprobs[row] = z.of(l.v[rank], r.top);
+    };
+    if (keep <= kThreads / 2) {
+        // mass up to each kept token in index order, by two threads
+        const int e = tid >> 1, half = tid & 1;
+        u64 w = 0, upto = 0;
+        if (e < keep) {
+            const int index = l.i[e];
+            w = l.weight[e];
+            for (int j = half; j < keep; j += 2)
+                if (l.i[j] <= index) upto += l.weight[j];
+        }
+        upto += __shfl_xor_sync(0xffffffffu, upto, 1);
+        if (half == 0 && upto > target && upto - w <= target) answer(e);
+        return;
     }
-    upto += __shfl_xor_sync(0xffffffffu, upto, 1);
-    if (half == 0 && upto > target && upto - w <= target) {
-        a.tokens[row] = index;
-        if (a.logprobs) a.logprobs[row] = z.of(l.ranked_v[e], r.top);
+    // by ranges of indices first: the mass of each, the one that holds the token, then its few tokens
+    u64* const range = reinterpret_cast<u64*>(sh.values.all);
+    const int shift = max(0, 32 - __clz(a.vocab - 1) - 9);  // at most kThreads = 2^9 ranges
+    range[tid] = 0;
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    for (int e = tid; e < keep; e += kThreads) atomicAdd(&range[l.i[e] >> shift], l.weight[e]);
+    __syncthreads();
+    const u64 in_range = range[tid], ahead = block_exclusive(in_range);
+    if (ahead <= target && target < ahead + in_range) sh.found_bin = tid, sh.bound[1] = ahead;
+    __syncthreads();
+    const int of = sh.found_bin;
+    for (int e = tid; e < keep; e += kThreads)
+        if (l.i[e] >> shift == of) sh.ordered_i[atomicAdd(&sh.listed, 1u)] = e;
+    __syncthreads();
+    const int few = int(sh.listed);
+    for (int e = tid; e < few; e += kThreads) {
+        const int rank = sh.ordered_i[e], index = l.i[rank];
+        u64 upto = sh.bound[1];
+        for (int j = 0; j < few; ++j)
+            if (l.i[sh.ordered_i[j]] <= index) upto += l.weight[sh.ordered_i[j]];
+        if (upto > target && upto - l.weight[rank] <= target) answer(rank);
     }
 }
 
@@ -1025,7 +1106,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
     const bool by_count = sh.found;
     int border = by_count ? sh.found_bin : INT_MAX;
     const u64 before = sh.bound[0], listed = sh.bound[1];
-    if (by_count && listed <= u64(kCap)) {
+    if (by_count && listed <= u64(kList)) {
         push_list(r, fmaxf(TY == 0 && border != kTinyBin ? near_edge(border) : bin_bottom(border), floor_v));
         cluster.sync();
         if (r.rank == 0) {
@@ -1076,7 +1157,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
             __syncthreads();
             border = sh.found_bin, ties = sh.bound[1];
             if (border == kTinyBin) return false;
-            if (sh.found <= kCap) {
+            if (sh.found <= kList) {
                 push_list(r, near_edge(border));
                 cluster.sync();
                 if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, whole);
@@ -1200,7 +1281,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
             const u64 counts_close = count_above(first, seen - count, cnt, close + 1);
             if (by_count) cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
             const float bottom = fmaxf(bin_bottom(close), floor_v);
-            const bool few = counts_close <= u64(kCap) && !by_count;
+            const bool few = counts_close <= u64(kList) && !by_count;
             if (few) push_list(r, bottom);
             const auto exact = [&](float at) {
                 const Pair* all = r.exchange(block_reduce(kept_mass(r, at), add_pairs));
@@ -1329,7 +1410,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     if (TY == 0 && a.part_rows)
         for (int i = tid; i < kCodes; i += kThreads) vectors()[i] = make_uint4(0, 0, 0, 0);  // kParts / 2 * 2 * kCodes words
     if (tid < 256) sh.pow256[tid] = exp2(frac - tid * (1.0 / 256));
-    if (tid == 0) sh.list.n = 0, sh.bound[0] = 0;
+    if (tid == 0) sh.listed = 0, sh.bound[0] = 0;
     __syncthreads();
     float top = -INFINITY;
     bool strange = false, masked = false;
