@@ -366,20 +366,32 @@ struct Row {
         }
         sum -= E * kRawZero;
     }
-    // The vectors of a warp: `steps` rows of 32, so that a slab, kStep of them, is a range of the row.
+    // The vectors of a warp: `steps` rows of 32, so that a slab, kStep of them, is a range of the row.  f(v, vector)
+    // for each, done(slab) by the whole warp after each slab.
     __device__ __forceinline__ int steps() const { return (nvec + 32 * kWarps - 1) / (32 * kWarps); }
-    template <class F>
-    __device__ __forceinline__ void each_step(F f) const {
-        const int n = steps(), from = (int(threadIdx.x) >> 5) * n * 32 + int(threadIdx.x & 31);
+    template <class F, class D>
+    __device__ __forceinline__ void each_slab(F f, D done) const {
+        static_assert(kStep % kAhead == 0, "whole batches");
+        const int n = steps(), warp_from = (int(threadIdx.x) >> 5) * n * 32, from = warp_from + int(threadIdx.x & 31);
 #pragma unroll 1
-        for (int s = 0; s < n; s += kAhead) {
-            uint4 q[kAhead];
+        for (int s = 0; s < n; s += kStep) {
+#pragma unroll 1
+            for (int b = s; b < min(s + kStep, n); b += kAhead) {
+                const int v = from + 32 * b, last = warp_from + 32 * (b + kAhead) - 1;
+                uint4 q[kAhead];
+                // a batch that lies in the row as a whole, the same for the warp
+                if (b + kAhead <= n && last < nvec && last != tail && warp_from + 32 * b != head) {
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (s + j < n && from + 32 * (s + j) < nvec) q[j] = vec(from + 32 * (s + j));
+                    for (int j = 0; j < kAhead; ++j) q[j] = resident ? vectors()[v + 32 * j] : __ldcg(source + v + 32 * j);
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (s + j < n) f(s + j, from + 32 * (s + j), q[j]);
+                    for (int j = 0; j < kAhead; ++j) f(v + 32 * j, q[j]);
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < kAhead; ++j)
+                        if (b + j < n && v + 32 * j < nvec) f(v + 32 * j, vec(v + 32 * j));
+                }
+            }
+            done(s / kStep);
         }
     }
 
@@ -566,19 +578,19 @@ __device__ int nth_equal(const Row<TY>& r, float value, u64 nth) {
     __syncthreads();  // slab may still be read
     if (threadIdx.x == 0) sh.found_bin = -1;
     uint32_t ties = 0;
-    r.each_step([&](int s, int v, const uint4& q) {
-        if (v < r.nvec && Elem<TY>::largest(q) >= value) {
+    r.each_slab(
+        [&](int v, const uint4& q) {
+            if (Elem<TY>::largest(q) < value) return;
             float x[E];
             Elem<TY>::unpack(q, x);
 #pragma unroll
             for (int e = 0; e < E; ++e) ties += x[e] == value && r.kept(value, v * E + e);
-        }
-        if (s % kStep == kStep - 1 || s == n - 1) {
+        },
+        [&](int slab) {
             ties = __reduce_add_sync(0xffffffffu, ties);
-            if (lane == 0) sh.slab[warp * each + s / kStep] = ties;
+            if (lane == 0) sh.slab[warp * each + slab] = ties;
             ties = 0;
-        }
-    });
+        });
     __syncthreads();
     if (nth > 0 && n > 0)
         find_value(r, 0, nth - 1, [&](float x, int slot) { return u64(x == value && r.kept(value, slot)); },
@@ -739,17 +751,15 @@ __device__ u64 slab_masses(const Row<TY>& r) {
     const float from = fmaxf(TIES ? r.tie_v : r.edge, r.weigh_from);
     u64 mine = 0, sum = 0, unused = 0;
     __syncthreads();  // slab may still be read
-    r.each_step([&](int s, int v, const uint4& q) {
-        if (v < r.nvec) r.template add_kept<TIES, false>(v, q, from, 0.f, sum, unused);
-        if (s % kStep == kStep - 1 || s == n - 1) {
-            if (__any_sync(0xffffffffu, sum != 0)) {
+    r.each_slab([&](int v, const uint4& q) { r.template add_kept<TIES, false>(v, q, from, 0.f, sum, unused); },
+                [&](int slab) {
+                    if (__any_sync(0xffffffffu, sum != 0)) {
 #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            }
-            if (lane == 0) shared().slab[warp * each + s / kStep] = sum;
-            mine += sum, sum = 0;
-        }
-    });
+                        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                    }
+                    if (lane == 0) shared().slab[warp * each + slab] = sum;
+                    mine += sum, sum = 0;
+                });
     return lane == 0 ? mine : 0;
 }
 template <int TY>
@@ -763,13 +773,10 @@ __device__ Pair kept_mass(const Row<TY>& r, float above) {
     Pair sum{0, 0};
     const bool ties = r.tie_i >= 0;
     const float from = fmaxf(ties ? r.tie_v : r.edge, r.weigh_from);
-    r.each_step([&](int, int v, const uint4& q) {
-        if (v >= r.nvec) return;
-        if (ties)
-            r.template add_kept<true, true>(v, q, from, above, sum.a, sum.b);
-        else
-            r.template add_kept<false, true>(v, q, from, above, sum.a, sum.b);
-    });
+    if (ties)
+        r.each_slab([&](int v, const uint4& q) { r.template add_kept<true, true>(v, q, from, above, sum.a, sum.b); }, [](int) {});
+    else
+        r.each_slab([&](int v, const uint4& q) { r.template add_kept<false, true>(v, q, from, above, sum.a, sum.b); }, [](int) {});
     return sum;
 }
 
@@ -1083,6 +1090,13 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
     const u64 limit = greedy ? 1 : k > 0 && k < a.vocab ? u64(k) : ~u64(0);
     if (greedy) p = 1.f;
 
+    if (a.vocab <= kList && (limit != ~u64(0) || p < 1.f)) {
+        push_list(r, fmaxf(bin_bottom(kValueBins - 1), floor_v));
+        cluster.sync();
+        if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, 0);
+        return true;
+    }
+
     // this thread's bins, largest values first; the border of top-k
     const int first = tid * kPerThread;
     uint32_t cnt[kPerThread];
@@ -1155,7 +1169,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
                 if (bin != kTinyBin) sh.bound[1] = ceil_div(target - sh.bound[1], w);
             }
             __syncthreads();
-            border = sh.found_bin, ties = sh.bound[1];
+            border = min(max(sh.found_bin, 0), kValueBins - 1), ties = sh.bound[1];
             if (border == kTinyBin) return false;
             if (sh.found <= kList) {
                 push_list(r, near_edge(border));
@@ -1431,15 +1445,15 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
                 const int part = TY == 0 && a.part_rows ? (b / kThreads + j) / a.part_rows : 0;
                 const uint32_t* const counts = TY == 0 && a.part_rows ? parts() + (part >> 1) * 2 * kCodes : h.own;
                 const uint32_t counts_at = uint32_t(__cvta_generic_to_shared(counts)), one = 1u << (16 * (part & 1));
-                bool plain = true;  // every value has a code
+                bool plain = true;  // every value has a code, or is -inf
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const uint32_t bits = __float_as_uint(x[e]), code = ((bits >> 16) & 0x7fffu) - kFirstCode;
                     const bool coded = code < uint32_t(kCodes);
                     add_where(coded, counts_at + 4 * (code + (bits >> 31) * kCodes), one);
-                    plain = plain & coded;
+                    plain = plain & (coded | x[e] == -INFINITY);
                 }
-                if (!plain) {  // a mask's -inf, mostly
+                if (!plain) {
                     bool others = false;
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
