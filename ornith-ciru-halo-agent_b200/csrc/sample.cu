@@ -343,10 +343,10 @@ struct Row {
             for (int i = 0; i < N; ++i) w[i] = x[i] >= weigh_from;
         }
     }
-    // Adds the kept mass of vector v, whose values are in q, to `sum` and that at `above` or higher to `part`.
+    // Adds the kept mass of vector v, whose values are in q, to `sum`, and that at low or high and above to two parts.
     // TIES: equal logits lie on both sides of the cut.  No value below `from` is kept.
-    template <bool TIES, bool PART>
-    __device__ __forceinline__ void add_kept(int v, const uint4& q, float from, float above, u64& sum, u64& part) const {
+    template <bool TIES, bool PARTS>
+    __device__ __forceinline__ void add_kept(int v, const uint4& q, float from, u64& sum, float low, float high, Pair& parts) const {
         if (El::largest(q) < from) return;
         float x[E];
         El::unpack(q, x);
@@ -355,14 +355,17 @@ struct Row {
         for (int e = 0; e < E; ++e) in[e] = TIES ? kept(x[e], v * E + e) && x[e] >= weigh_from : x[e] >= from;
         if (count_mode) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum += in[e], part += PART && in[e] && x[e] >= above;
+            for (int e = 0; e < E; ++e) sum += in[e];
             return;
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const u64 raw = raw_weight(x[e], in[e]);
             sum += raw;
-            if (PART) part += x[e] >= above ? raw - kRawZero : 0;
+            if (PARTS) {
+                parts.a += x[e] >= low ? raw - kRawZero : 0;
+                parts.b += x[e] >= high ? raw - kRawZero : 0;
+            }
         }
         sum -= E * kRawZero;
     }
@@ -612,44 +615,12 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
     float scale = 0.f;               // of the last histogram
     int border = -1;                 // its bin, where there was one
     auto bin = [&](float x) { return max(0, min(kBins - 1, __float2int_rz(__fmul_rn(__fsub_rn(hi, x), scale)))); };
+    // Few logits lie in the range once it is narrow: one branch for the others.
     auto inside = [&](float x, int slot) {
-        return x >= lo && x <= hi && r.kept(x, slot) && (border < 0 || bin(x) == border);
+        return (x >= lo & x <= hi) && r.kept(x, slot) && (border < 0 || bin(x) == border);
     };
     while (n > u64(kCap)) {
-        // the values left: all alike, or split
-        float mn = INFINITY, mx = -INFINITY;
-        r.each([&](float x, int slot) {
-            if (inside(x, slot)) mn = fminf(mn, x), mx = fmaxf(mx, x);
-        });
-        auto range = [](Pair p, Pair q) {
-            return Pair{as_bits(fminf(as_float(p.a), as_float(q.a))), as_bits(fmaxf(as_float(p.b), as_float(q.b)))};
-        };
-        Pair own = block_reduce(Pair{as_bits(mn), as_bits(mx)}, range);
-        const Pair* all = r.exchange(own);
-        for (int q = 0; q < r.size; ++q) own = range(own, all[q]);
-        lo = as_float(own.a), hi = as_float(own.b), border = -1;
-        if (!(lo < hi)) {
-            if (lo > hi) return;  // none
-            // equal logits: the lowest indices are kept
-            u64 need = target - base;
-            if (MASS) {
-                const u64 w = r.weight(hi);
-                if (w == 0) return;
-                need = ceil_div(need, w);
-            }
-            u64 ties = 0;
-            r.each([&](float x, int slot) { ties += inside(x, slot); });
-            auto add = [](Pair p, Pair q) { return Pair{p.a + q.a, 0}; };
-            all = r.exchange(block_reduce(Pair{ties, 0}, add));
-            u64 ahead = 0;
-            for (int q = 0; q < r.rank; ++q) ahead += all[q].a;
-            const int mine = nth_equal(r, hi, ahead < need ? need - ahead : 0);
-            all = r.exchange(Pair{u64(uint32_t(mine)), 0});
-            int index = -1;
-            for (int q = 0; q < r.size; ++q) index = max(index, int(uint32_t(all[q].a)));
-            if (index >= 0) r.cut_at(hi, index);
-            return;
-        }
+        border = -1;
         scale = __fdiv_rn(float(kBins), __fsub_rn(hi, lo));
         for (int b = threadIdx.x; b < kBins; b += kThreads) {
             f.cnt[b] = f.tcnt[b] = 0;
@@ -697,6 +668,41 @@ __device__ void cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
         border = sh.found_bin, base = sh.bound[1];
         n = f.tcnt[border];
         __syncthreads();  // found is written again
+        if (n <= u64(kCap)) break;
+        // the values left: all alike, or split
+        float mn = INFINITY, mx = -INFINITY;
+        r.each([&](float x, int slot) {
+            if (inside(x, slot)) mn = fminf(mn, x), mx = fmaxf(mx, x);
+        });
+        auto range = [](Pair p, Pair q) {
+            return Pair{as_bits(fminf(as_float(p.a), as_float(q.a))), as_bits(fmaxf(as_float(p.b), as_float(q.b)))};
+        };
+        Pair own = block_reduce(Pair{as_bits(mn), as_bits(mx)}, range);
+        const Pair* all = r.exchange(own);
+        for (int q = 0; q < r.size; ++q) own = range(own, all[q]);
+        lo = as_float(own.a), hi = as_float(own.b), border = -1;
+        if (!(lo < hi)) {
+            if (lo > hi) return;  // none
+            // equal logits: the lowest indices are kept
+            u64 need = target - base;
+            if (MASS) {
+                const u64 w = r.weight(hi);
+                if (w == 0) return;
+                need = ceil_div(need, w);
+            }
+            u64 ties = 0;
+            r.each([&](float x, int slot) { ties += inside(x, slot); });
+            auto add = [](Pair p, Pair q) { return Pair{p.a + q.a, 0}; };
+            all = r.exchange(block_reduce(Pair{ties, 0}, add));
+            u64 ahead = 0;
+            for (int q = 0; q < r.rank; ++q) ahead += all[q].a;
+            const int mine = nth_equal(r, hi, ahead < need ? need - ahead : 0);
+            all = r.exchange(Pair{u64(uint32_t(mine)), 0});
+            int index = -1;
+            for (int q = 0; q < r.size; ++q) index = max(index, int(uint32_t(all[q].a)));
+            if (index >= 0) r.cut_at(hi, index);
+            return;
+        }
     }
     // rank the tokens left exactly; the exchange before tells every CTA that nobody reads the lists any more
     r.exchange(Pair{0, 0});
@@ -749,9 +755,10 @@ template <int TY, bool TIES>
 __device__ u64 slab_masses(const Row<TY>& r) {
     const int n = r.steps(), each = slabs_of_warp(n), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float from = fmaxf(TIES ? r.tie_v : r.edge, r.weigh_from);
-    u64 mine = 0, sum = 0, unused = 0;
+    u64 mine = 0, sum = 0;
+    Pair none{0, 0};
     __syncthreads();  // slab may still be read
-    r.each_slab([&](int v, const uint4& q) { r.template add_kept<TIES, false>(v, q, from, 0.f, sum, unused); },
+    r.each_slab([&](int v, const uint4& q) { r.template add_kept<TIES, false>(v, q, from, sum, 0.f, 0.f, none); },
                 [&](int slab) {
                     if (__any_sync(0xffffffffu, sum != 0)) {
 #pragma unroll
@@ -767,16 +774,17 @@ __device__ u64 slab_masses(const Row<TY>& r) {
     return r.tie_i < 0 ? slab_masses<TY, false>(r) : slab_masses<TY, true>(r);
 }
 
-// The kept mass of this CTA, and that at `above` or higher, in this thread's vectors.
-template <int TY>
-__device__ Pair kept_mass(const Row<TY>& r, float above) {
-    Pair sum{0, 0};
+// The kept mass in this thread's vectors, and that at low or high and above (by mass, not by number).
+template <int TY, bool PARTS>
+__device__ u64 kept_mass(const Row<TY>& r, float low, float high, Pair& parts) {
+    u64 sum = 0;
+    parts = Pair{0, 0};
     const bool ties = r.tie_i >= 0;
     const float from = fmaxf(ties ? r.tie_v : r.edge, r.weigh_from);
     if (ties)
-        r.each_slab([&](int v, const uint4& q) { r.template add_kept<true, true>(v, q, from, above, sum.a, sum.b); }, [](int) {});
+        r.each_slab([&](int v, const uint4& q) { r.template add_kept<true, PARTS>(v, q, from, sum, low, high, parts); }, [](int) {});
     else
-        r.each_slab([&](int v, const uint4& q) { r.template add_kept<false, true>(v, q, from, above, sum.a, sum.b); }, [](int) {});
+        r.each_slab([&](int v, const uint4& q) { r.template add_kept<false, PARTS>(v, q, from, sum, low, high, parts); }, [](int) {});
     return sum;
 }
 
@@ -1297,28 +1305,22 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
             const float bottom = fmaxf(bin_bottom(close), floor_v);
             const bool few = counts_close <= u64(kList) && !by_count;
             if (few) push_list(r, bottom);
-            const auto exact = [&](float at) {
-                const Pair* all = r.exchange(block_reduce(kept_mass(r, at), add_pairs));
-                Pair sums{0, 0};
-                for (int q = 0; q < r.size; ++q) sums = add_pairs(sums, all[q]);
-                return sums;
-            };
-            const Pair mass = exact(bottom);
+            // the exact masses: of all, of the bins up to the last, above the first
+            const float edge = bin_top(open);
+            Pair parts;
+            const u64 own = kept_mass<TY, true>(r, bottom, nextafterf(edge, INFINITY), parts);
+            const Pair* all = r.exchange(block_reduce(Pair{own, parts.a}, add_pairs));
+            Pair mass{0, 0};
+            for (int q = 0; q < r.size; ++q) mass = add_pairs(mass, all[q]);
             const u64 target = nucleus(mass.a, p);
             const bool low_enough = mass.b >= target;
             if (few && low_enough) {
                 if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, mass.a);
                 return true;
             }
-            const float edge = bin_top(open);
-            Row<TY> upper = r;  // what lies above the first bin
-            upper.keep_from(fmaxf(nextafterf(edge, INFINITY), r.edge));
-            const u64 base = [&] {
-                const Pair* all = r.exchange(block_reduce(kept_mass(upper, INFINITY), add_pairs));
-                u64 sum = 0;
-                for (int q = 0; q < r.size; ++q) sum += all[q].a;
-                return sum;
-            }();
+            all = r.exchange(block_reduce(Pair{parts.b, 0}, add_pairs));
+            u64 base = 0;
+            for (int q = 0; q < r.size; ++q) base += all[q].a;
             const bool high_enough = base < target;
             cut_row<TY, true>(r, low_enough ? bottom : r.weigh_from, high_enough ? edge : r.top, high_enough ? base : 0, target,
                               low_enough && high_enough ? counts_close - counts_open : a.vocab);
@@ -1561,7 +1563,8 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         if (by_mass) {
             const bool counted = r.count_mode;
             r.weigh(false, frac, T);  // the nucleus goes by mass for u = 0 too
-            all = r.exchange(block_reduce(kept_mass(r, top), add_pairs));
+            Pair none;
+            all = r.exchange(block_reduce(Pair{kept_mass<TY, false>(r, 0.f, 0.f, none), 0}, add_pairs));
             u64 mass = 0;
             for (int i = 0; i < size; ++i) mass += all[i].a;
             cut_row<TY, true>(r, from(37.0), top, 0, nucleus(mass, p), a.vocab);
