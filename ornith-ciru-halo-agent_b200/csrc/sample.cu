@@ -54,9 +54,9 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kMaxVocab = 1 << 19, kSms = 148;
 constexpr int kBins = 1024, kCap = 256, kList = 2 * kThreads;  // bins of a search, candidates it ranks, tokens of a list
 constexpr int kAhead = 4;                                      // vectors of a thread in flight
-constexpr int kMaxVecs = 60 * kThreads, kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
+constexpr int kParts = 4, kPartVecs = 255 * 32, kMaxVecs = kParts * kPartVecs, kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
 // 16-byte vectors of a CTA: at most, and kept on chip by one or two CTAs of an SM
-constexpr int kParts = 4;  // of a bf16 CTA's logits that do not stay on chip, counted apart in 16 bits: 15 * kThreads * 8 < 2^16
+// Parts of a bf16 CTA's logits that do not stay on chip, counted apart in 16 bits: kPartVecs * 8 < 2^16.
 constexpr int kStep = 8, kSlabs = kMaxVecs / 32 / kStep + kWarps;  // rows of 32 vectors in a slab; slabs of a CTA
 constexpr float kMaxTemperature = 1e30f;
 constexpr uint32_t kFlagNonfinite = 1, kFlagParameter = 2, kFlagNothingLeft = 4;
@@ -71,7 +71,7 @@ struct Args {
     uint32_t* flags;
     int vocab, vecs;  // vecs: 16-byte vectors of a row for one CTA
     int resident;     // they stay in shared memory
-    int part_rows;    // bf16: rows of kThreads vectors in a part that is counted apart, or 0
+    int part_vecs;    // bf16: vectors (a multiple of 32) of a part that is counted apart, or 0
 };
 
 template <int TY>
@@ -810,6 +810,23 @@ __device__ void write_token(const Row<TY>& r, const Args& a, int row, u64 ahead,
 __device__ __forceinline__ Pair add_floats(Pair p, Pair q) {
     return Pair{as_bits(__fadd_rn(as_float(p.a), as_float(q.a))), as_bits(__fadd_rn(as_float(p.b), as_float(q.b)))};
 }
+// This CTA's logits equal to `top`, counted, and the others' exp(x - top),
+// summed: vector by vector, so that no sum has more than some 70 steps.
+template <int TY>
+__device__ Pair exponentials(const Row<TY>& r, float top) {
+    float equal = 0.f, others = 0.f;
+    r.each_vector([&](int, const uint4& q) {
+        float x[Elem<TY>::E], sum = 0.f;
+        Elem<TY>::unpack(q, x);
+#pragma unroll
+        for (int e = 0; e < Elem<TY>::E; ++e) {
+            equal += x[e] == top ? 1.f : 0.f;
+            sum += x[e] == top ? 0.f : expf(__fsub_rn(x[e], top));
+        }
+        others += sum;
+    });
+    return block_reduce(Pair{as_bits(equal), as_bits(others)}, add_floats);
+}
 __device__ __forceinline__ Pair add_pairs(Pair p, Pair q) { return Pair{p.a + q.a, p.b + q.b}; }
 
 // floor(u * mass): the token is the first whose running mass is above it.
@@ -1217,7 +1234,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         Partition z{1.f, 0.f};
         if (a.logprobs) z = counted_partition(r);
         u64 target_at = ahead;
-        if (a.part_rows) {
+        if (a.part_vecs) {
             // the part that holds it, by the parts' counts
             u64 of[kParts] = {0, 0, 0, 0};
 #pragma unroll 1
@@ -1253,8 +1270,8 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
 #pragma unroll
             for (int q = 0; q < kParts - 1; ++q)
                 if (part == q && target_at + sums[q] <= target) target_at += sums[q], part = q + 1;
-            const int from = part * a.part_rows * kThreads;
-            r.narrow(from, min(a.part_rows * kThreads, r.nvec - from));
+            const int from = part * a.part_vecs;
+            r.narrow(from, min(a.part_vecs, r.nvec - from));
             if (border != INT_MAX) here = sh.part_here[part], mine = sh.part_kept[part];
         }
         if (border == kTinyBin) {
@@ -1332,12 +1349,15 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
     }
 }
 
-// *shared += v where `in`, without a branch: eight of them in a row would each
-// part and join the warp again.
-__device__ __forceinline__ void add_where(bool in, uint32_t shared_address, uint32_t v) {
-    asm volatile("{ .reg .pred p; setp.ne.u32 p, %0, 0; @p red.shared.add.u32 [%1], %2; }" ::"r"(uint32_t(in)),
-                 "r"(shared_address), "r"(v)
+// *shared += v where offset < 4 kCodes, without a branch: eight of them in a
+// row would each part and join the warp again.
+__device__ __forceinline__ void add_coded(uint32_t offset, uint32_t shared_address, uint32_t v) {
+    asm volatile("{ .reg .pred p; setp.lt.u32 p, %0, %3; @p red.shared.add.u32 [%1], %2; }" ::"r"(offset), "r"(shared_address),
+                 "r"(v), "n"(4 * kCodes)
                  : "memory");
+}
+__device__ __forceinline__ void add_shared(uint32_t shared_address, uint32_t v) {
+    asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(shared_address), "r"(v) : "memory");
 }
 
 // The values of a counted vector above -128 that have no code.  1: NaN or
@@ -1365,6 +1385,64 @@ __device__ __noinline__ uint32_t note_others(const uint4 q, int part) {
         }
     }
     return notes;
+}
+
+// The notes of a vector that has values without a code.
+template <int TY>
+__device__ __forceinline__ uint32_t classify(const uint4& q, const float* x, int part) {
+    bool others = false, masked = false;
+#pragma unroll
+    for (int e = 0; e < Elem<TY>::E; ++e) {
+        others = others | !(fabsf(x[e]) >= 0x1p-10f & x[e] < 128.f);
+        masked = masked | (x[e] <= -128.f & x[e] > -INFINITY);
+    }
+    return (others ? note_others<TY>(q, part) : 0) | uint32_t(masked) << 2;
+}
+
+// 4 kCodes where a half of the word is negative, else 0: the half's sign in all bits (byte 1's or byte 3's, by the
+// replicating mode of prmt), multiplied, as the multiplier has less to do here than the integer unit.
+template <int SELECTOR>
+__device__ __forceinline__ uint32_t negative_offset(uint32_t word) {
+    uint32_t sign;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(sign) : "r"(word), "n"(SELECTOR));
+    return sign * uint32_t(-4 * kCodes);
+}
+
+// Counts eight bf16 values by their bits.  Whether all have a code is asked of
+// pairs (magnitude - kFirstCode < kCodes); a warp of which all have adds eight
+// times five instructions a value, any other one tests each value.
+__device__ __forceinline__ uint32_t count_pairs(const uint4& q, int part, const uint32_t* counts, uint32_t one) {
+    constexpr uint32_t kPair = 0x10001u, kMagnitude = 0x7fff * kPair, kShift = (0x10000u - kFirstCode) * kPair;
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    const uint32_t at = uint32_t(__cvta_generic_to_shared(counts));
+    const auto above = [](uint32_t pair) { return max(pair & 0xffffu, pair >> 16) >= uint32_t(kCodes); };
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = __viaddmax_u16x2(w[i] & kMagnitude, kShift, most);
+    if (!__any_sync(__activemask(), above(most))) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t low = 4 * (w[i] & 0x7fffu) + (at - 4 * kFirstCode);
+            const uint32_t high = ((w[i] & 0x7fff0000u) >> 14) + (at - 4 * kFirstCode);
+            add_shared(low + negative_offset<0x9999>(w[i]), one);
+            add_shared(high + negative_offset<0xbbbb>(w[i]), one);
+        }
+        return 0;
+    }
+    // the same with -inf as 2 - 2^-7, and every value tested
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t infinite = __heq2_mask(reinterpret_cast<const __nv_bfloat162&>(w[i]), __float2bfloat162_rn(-INFINITY));
+        most = __viaddmax_u16x2((w[i] & kMagnitude & ~infinite) | (infinite & 0x3fff * kPair), kShift, most);
+        const uint32_t low = 4 * (w[i] & 0x7fffu) - 4 * kFirstCode, high = ((w[i] & 0x7fff0000u) >> 14) - 4 * kFirstCode;
+        add_coded(low, low + at + negative_offset<0x9999>(w[i]), one);
+        add_coded(high, high + at + negative_offset<0xbbbb>(w[i]), one);
+    }
+    if (!above(most)) return 0;
+    float x[8];
+    Elem<0>::unpack(q, x);
+    return classify<0>(q, x, part);
 }
 
 // One cluster per row.  The barrier of a cluster is the hardware's: all its
@@ -1423,13 +1501,13 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
         for (int i = tid; i < int(sizeof(h.all) / 16); i += kThreads) reinterpret_cast<uint4*>(h.all)[i] = make_uint4(0, 0, 0, 0);
     }
     const int frac = min(51, 62 - (32 - __clz((a.vocab - 1) | 1)));  // s
-    if (TY == 0 && a.part_rows)
+    if (TY == 0 && a.part_vecs)
         for (int i = tid; i < kCodes; i += kThreads) vectors()[i] = make_uint4(0, 0, 0, 0);  // kParts / 2 * 2 * kCodes words
     if (tid < 256) sh.pow256[tid] = exp2(frac - tid * (1.0 / 256));
     if (tid == 0) sh.listed = 0, sh.bound[0] = 0;
     __syncthreads();
     float top = -INFINITY;
-    bool strange = false, masked = false;
+    bool strange = false;
     uint32_t notes = 0;  // of note_others
     for (int b = 0; b < nvec; b += kBatch * kThreads) {
         uint4 now[kBatch];
@@ -1441,32 +1519,26 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
             const int v = b + j * kThreads + tid;
             if (v >= nvec) break;
             if (resident) vectors()[v] = now[j];
-            float x[E];
-            El::unpack(now[j], x);
-            if (counting) {
-                const int part = TY == 0 && a.part_rows ? (b / kThreads + j) / a.part_rows : 0;
-                const uint32_t* const counts = TY == 0 && a.part_rows ? parts() + (part >> 1) * 2 * kCodes : h.own;
-                const uint32_t counts_at = uint32_t(__cvta_generic_to_shared(counts)), one = 1u << (16 * (part & 1));
-                bool plain = true;  // every value has a code, or is -inf
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const uint32_t bits = __float_as_uint(x[e]), code = ((bits >> 16) & 0x7fffu) - kFirstCode;
-                    const bool coded = code < uint32_t(kCodes);
-                    add_where(coded, counts_at + 4 * (code + (bits >> 31) * kCodes), one);
-                    plain = plain & (coded | x[e] == -INFINITY);
-                }
-                if (!plain) {
-                    bool others = false;
+            if (TY == 0) {
+                const int part = a.part_vecs ? (v >= a.part_vecs) + (v >= 2 * a.part_vecs) + (v >= 3 * a.part_vecs) : 0;
+                notes |= count_pairs(now[j], part, a.part_vecs ? parts() + (part >> 1) * 2 * kCodes : h.own, 1u << (16 * (part & 1)));
+            } else {
+                float x[E];
+                El::unpack(now[j], x);
+                if (counting) {
+                    const uint32_t counts_at = uint32_t(__cvta_generic_to_shared(h.own));
+                    bool plain = true;  // every value has a code, or is -inf
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        others = others | !(fabsf(x[e]) >= 0x1p-10f & x[e] < 128.f);
-                        masked = masked | (x[e] <= -128.f & x[e] > -INFINITY);
+                        const uint32_t bits = __float_as_uint(x[e]), code = ((bits >> 16) & 0x7fffu) - kFirstCode;
+                        add_coded(4 * code, counts_at + 4 * (code + (bits >> 31) * kCodes), 1u);
+                        plain = plain & (code < uint32_t(kCodes) | x[e] == -INFINITY);
                     }
-                    if (others) notes |= note_others<TY>(now[j], part);
-                }
-            } else {
+                    if (!plain) notes |= classify<TY>(now[j], x, 0);
+                } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) strange = strange | !(x[e] < INFINITY);
+                    for (int e = 0; e < E; ++e) strange = strange | !(x[e] < INFINITY);
+                }
             }
             top = fmaxf(top, El::largest(now[j]));
         }
@@ -1474,8 +1546,8 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
 
     Row<TY> r{resident, head, tail, base, begin, a.vocab, nvec, i_first, rank, size, 0};
     auto join = [](Pair x, Pair y) { return Pair{as_bits(fmaxf(as_float(x.a), as_float(y.a))), x.b | y.b}; };
-    const Pair mine = block_reduce(Pair{as_bits(top), notes | uint32_t(strange) | uint32_t(masked) << 2}, join);
-    if (TY == 0 && a.part_rows)
+    const Pair mine = block_reduce(Pair{as_bits(top), notes | uint32_t(strange)}, join);
+    if (TY == 0 && a.part_vecs)
         for (int i = tid; i < 2 * kCodes; i += kThreads) {
             uint32_t c = 0;
 #pragma unroll
@@ -1488,13 +1560,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     Pair sums{0, 0};
     if (TY != 0 && a.logprobs && !from_mass) {
         const float local = as_float(mine.a);
-        float equal = 0.f, others = 0.f;
-        r.each([&](float x, int) {
-            const float e = expf(__fsub_rn(x, local));
-            equal += x == local ? 1.f : 0.f;
-            others += x == local ? 0.f : e;
-        });
-        sums = block_reduce(Pair{as_bits(equal), as_bits(others)}, add_floats);
+        sums = exponentials(r, local);
     }
     cluster.barrier_wait();
     const uint32_t own_tiny = counting ? h.own[2 * kCodes] : 0;
@@ -1533,13 +1599,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
 
     // The general way: rows without a cut, and those that the counts do not tell enough about.
     if (TY == 0 && a.logprobs) {
-        float equal = 0.f, others = 0.f;
-        r.each([&](float x, int) {
-            const float e = expf(__fsub_rn(x, top));
-            equal += x == top ? 1.f : 0.f;
-            others += x == top ? 0.f : e;
-        });
-        const Pair own = block_reduce(Pair{as_bits(equal), as_bits(others)}, add_floats);
+        const Pair own = exponentials(r, top);
         if (tid < size) *cluster.map_shared_rank(&sh.part[rank], tid) = Pair{as_bits(top), own.a | own.b << 32};
         cluster.sync();
     }
@@ -1640,8 +1700,8 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(M) * unsigned(size));
     cfg.blockDim = dim3(kThreads);
-    a.part_rows = type == 0 && !a.resident && a.vecs >= kParts * kThreads ? ((a.vecs + kThreads - 1) / kThreads + kParts - 1) / kParts : 0;
-    cfg.dynamicSmemBytes = sizeof(Shared) + (a.resident ? size_t(a.vecs) * 16 : a.part_rows ? size_t(kCodes) * 16 : 0);
+    a.part_vecs = type == 0 && !a.resident && a.vecs >= kParts * kThreads ? (a.vecs + 32 * kParts - 1) / (32 * kParts) * 32 : 0;
+    cfg.dynamicSmemBytes = sizeof(Shared) + (a.resident ? size_t(a.vecs) * 16 : a.part_vecs ? size_t(kCodes) * 16 : 0);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -2,9 +2,11 @@
 
 Tokens are compared exactly: the weights' relative error (below 1e-13) moves a
 border between two tokens past a given random number with a probability below
-1e-9 a row.  A log probability is off by the sum of at most 68 fp32 terms in a
-thread, each exact to two steps (72 steps of 2^-24 relative in all, the same
-absolutely after the logarithm), and by half a step of its own."""
+1e-9 a row.  A log probability is off by its fp32 sum: exponentials exact to two
+steps (4 of 2^-24), up to 8 + 60 additions in a thread (4 + 20 at the sizes
+here), 9 over a block, 5 over a cluster and 2 steps of the logarithm - at most
+72 of 2^-24 relative here, the same absolutely after the logarithm - and by half
+a step of its own."""
 import importlib
 import math
 
@@ -110,12 +112,55 @@ def test_settings(native, dtype, head):
 
 
 @pytest.mark.parametrize('m,vocab,dtype', [(1, 248320, BF16), (2, 248320, FP32), (20, 248320, BF16),
-                                           (1, 524288, FP32), (2, 524287, FP16), (70, 65536, FP32), (500, 256, BF16)])
+                                           (1, 524288, FP32), (2, 524287, FP16), (1, 500000, FP32),
+                                           (70, 65536, FP32), (500, 256, BF16), (160, 40000, FP32), (300, 30000, BF16)])
 def test_sizes(native, m, vocab, dtype):
     """One to sixteen CTAs a row, with rows enough to fill the GPU and without."""
     x = logits_of(m, vocab, dtype, 3, head=64)
     for i, s in enumerate((dict(), dict(T=0.8, k=40, p=0.95), dict(T=2.0, p=0.9), dict(T=1.2, k=20000, min_p=1e-6))):
         check(native, x, u=uniform(m, i), **s)
+
+
+def test_lists_of_every_length(native):
+    """Kept sets around the sizes where one CTA ranks them (a few, half a list, a whole one) and beyond."""
+    for dtype in (BF16, FP16, FP32):
+        x = logits_of(2, 100003, dtype, 21, spread=1.0)
+        for i, k in enumerate((2, 100, 255, 256, 257, 700, 1023, 1024, 1025, 3000)):
+            check(native, x, k=k, u=uniform(2, i))
+            check(native, x, T=1.7, k=k, p=0.9, u=uniform(2, 50 + i))
+        peaked = logits_of(2, 100003, dtype, 22, head=1500)
+        for i, p in enumerate((0.3, 0.6, 0.8, 0.9, 0.95, 0.99, 0.999)):
+            check(native, peaked, T=1.0, p=p, u=uniform(2, i))
+
+
+def test_estimates_that_fail(native):
+    """Nucleus borders where a bin's middle says little of its mass: few heavy tokens at a bin's edge."""
+    for dtype in (FP16, FP32):
+        x = torch.full((4, 30000), -3.0)
+        x[0, 17::1000] = 16.01                         # thirty equal tokens at the bottom of a wide bin
+        x[1, 5], x[1, 6:300] = 63.99, 63.6             # one at the top of a bin, others below
+        x[2, :20000] = 8.0 + torch.arange(20000) / 1e5  # one bin holds nearly everything
+        x[3, ::2] = 1.0
+        x = x.to(dtype).to(DEV)
+        for i, p in enumerate((0.1, 0.5, 0.75, 0.9, 0.97)):
+            for T in (0.3, 1.0, 2.5):
+                check(native, x, T=T, p=p, u=uniform(4, i))
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+def test_values_outside_the_counted_range(native, dtype):
+    """Logits of 128 and more, of -128 and less that still have a weight, and near zero, also on a border."""
+    base = logits_of(6, 9001, dtype, 31, spread=1.0)
+    x = base.clone()
+    x[0] += 200.0
+    x[1, ::3] = -300.0
+    x[2, 4000] = 127.5
+    x[3] = (base[3].float() * 2.0 ** -11).to(dtype)            # all below 2^-10 but a few
+    x[4, 100:130] = torch.linspace(-9e-4, 9e-4, 30, device=DEV).to(dtype)
+    x[5] = torch.where(base[5] > 0.5, base[5], 0.0 * base[5])  # half of the row is 0 or -0
+    for i, s in enumerate((dict(), dict(T=100.0), dict(T=100.0, k=3500), dict(T=50.0, p=0.6), dict(k=4400), dict(k=4510),
+                           dict(p=0.4), dict(p=0.75), dict(T=0.0), dict(T=20.0, min_p=0.9), dict(min_p=0.999))):
+        check(native, x, u=uniform(6, i), **s)
 
 
 def test_row_parameters(native):
