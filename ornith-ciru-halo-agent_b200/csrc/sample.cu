@@ -19,18 +19,29 @@
 // table driven (Tang, 1989): 2^-n/256 from a table of 256 values times a Taylor
 // polynomial of degree 3 in the remainder (at most ln 2 / 512, so 2e-13 off).
 //
-// Layout of the work.  A cluster of 1 to 16 CTAs takes one row: every CTA
-// keeps its share of the logits in shared memory, so the row is read from HBM
-// once, however many steps the selection takes.  While the logits come in, a
-// CTA counts them by their leading 16 bits (a bf16's own value); the merged
-// counts say where a cut lies.  From there:
+// Layout of the work.  A cluster of 1 to 16 CTAs takes one row, a CTA one
+// contiguous share.  The row is read from HBM once: a small share then stays
+// in shared memory, later passes over a large one find it in L2.  While the
+// logits come in, a CTA counts them by their leading 16 bits (a bf16's own
+// value); the merged counts say where a cut lies.  From there:
+//   - where at most kList tokens can be kept, they are pushed to the first CTA,
+//     which ranks them and draws;
 //   - a bf16 row is known but for its order: masses are counts times weights,
-//     a cut is a value and a number of equal logits;
-//   - for fp16 and fp32 the counts bound the masses, and only the tokens of the
-//     bins that can hold the border are looked at one by one;
-//   - where at most 256 tokens can be kept, one CTA ranks and draws among them;
-//     else each CTA weighs its kept tokens and the one that holds the drawn
-//     token finds it.
+//     a cut is a value and a number of equal logits, and only the slab that
+//     holds the drawn token is weighed (of a large share first the quarter,
+//     by counts that are kept apart for each);
+//   - for fp16 and fp32 the counts bound the masses, and the tokens of the bins
+//     that can hold the border are weighed one by one;
+//   - uncut fp16 and fp32 rows, and those that the counts do not hold (many
+//     tiny values, a largest logit outside +-128), search by bins of value.
+//
+// What bounds it.  Not HBM (64 uncut fp32 rows of 248320 take 40.0 us, 1.59
+// TB/s): the small cases wait for some ten steps between the CTAs of a row
+// (17 us for one row), the large ones for the shared-memory counts, a weight's
+// double-precision arithmetic and instruction issue.  Measured: a count of a
+// bf16 row's logits issues at 2.6 instructions a clock; weights take 7.2 clocks
+// for a warp's 32; 256 bf16 rows with a nucleus of many thousand tokens take
+// 111 us (1.15 TB/s) against 729 with a weight for every logit.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -52,11 +63,16 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kMaxVocab = 1 << 19, kSms = 148;
-constexpr int kBins = 1024, kCap = 256, kList = 2 * kThreads;  // bins of a search, candidates it ranks, tokens of a list
-constexpr int kAhead = 4;                                      // vectors of a thread in flight
-constexpr int kParts = 4, kPartVecs = 255 * 32, kMaxVecs = kParts * kPartVecs, kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
-// 16-byte vectors of a CTA: at most, and kept on chip by one or two CTAs of an SM
-// Parts of a bf16 CTA's logits that do not stay on chip, counted apart in 16 bits: kPartVecs * 8 < 2^16.
+// Bins of a search, candidates that it ranks; tokens of a list: 19 us against 24 with 256 for 7 rows of 4099.
+constexpr int kBins = 1024, kCap = 256, kList = 2 * kThreads;
+// Vectors of a thread in flight: 111 us for 256 rows of 248320 with four, 113 with two.
+constexpr int kAhead = 4;
+// Parts of a bf16 CTA's logits that do not stay on chip, counted apart in 16 bits (kPartVecs * 8 < 2^16), so that the
+// drawn token is sought in one of them: 111 us against 206 for 256 rows of 248320, 44 against 56 for 64.
+constexpr int kParts = 4, kPartVecs = 255 * 32, kMaxVecs = kParts * kPartVecs;
+// 16-byte vectors that one CTA or two of an SM keep on chip.  Where both fit, 19.4 us against 20.3 from L2 for 7 rows
+// of 4099; 8192 for two, which leaves one CTA on an SM: 67 us against 44 for 64 rows.
+constexpr int kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
 constexpr int kStep = 8, kSlabs = kMaxVecs / 32 / kStep + kWarps;  // rows of 32 vectors in a slab; slabs of a CTA
 constexpr float kMaxTemperature = 1e30f;
 constexpr uint32_t kFlagNonfinite = 1, kFlagParameter = 2, kFlagNothingLeft = 4;
@@ -1666,8 +1682,10 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     }
     // A row may start inside a 16-byte vector and then takes one more.
     const int total_vecs = (vocab + per_vec - 1 + per_vec - 1) / per_vec;
-    // CTAs a row: as many as run at once (two on each SM), as the steps between two passes over the logits take
-    // much the same time for a large share as for a small one; no share below 4 KB, none above kMaxVecs.
+    // CTAs a row: the largest power of two that runs at once (two on each SM), as the steps between two passes over
+    // the logits take much the same time for a large share as for a small one: 44 us for 64 mixed rows against 56 with
+    // half as many and 61 with twice, 111 against 127 with twice for 256.  No share above kMaxVecs; none below 4 KB
+    // (1 and 16 KB measure the same).
     int size = 1;
     while (size < kMaxCluster && ((total_vecs + size - 1) / size > kMaxVecs ||
                                   (int64_t(M) * size * 2 <= 2 * kSms && total_vecs / size > 512)))

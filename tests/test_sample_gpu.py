@@ -147,6 +147,26 @@ def test_estimates_that_fail(native):
                 check(native, x, T=T, p=p, u=uniform(4, i))
 
 
+@pytest.mark.parametrize('vocab', [261113, 261114])
+def test_largest_shares_of_equal_logits(native, vocab):
+    """One CTA takes as many bf16 logits as its four counts of 16 bits hold, and one more takes two CTAs."""
+    x = torch.full((150, vocab), 1.5, dtype=BF16, device=DEV)
+    x[1::4, ::2] = -2.0
+    x[2::4, 65280:] = -float('inf')
+    x[3::4, :-5] = -float('inf')
+    for i, s in enumerate((dict(), dict(p=0.9), dict(k=200000), dict(T=2.0, p=0.3))):
+        check(native, x, u=uniform(150, i), **s)
+
+
+def test_rows_further_apart_than_32_bits(native):
+    vocab, stride = 70001, 2 ** 31 + 17
+    for dtype in (BF16, FP16):
+        x = torch.empty(2 * stride + vocab, dtype=dtype, device=DEV).as_strided((3, vocab), (stride, 1))
+        x.copy_(logits_of(3, vocab, dtype, 41, head=64))
+        for i, s in enumerate((dict(), dict(k=30, p=0.9), dict(p=0.99), dict(T=0.0))):
+            check(native, x, u=uniform(3, i), **s)
+
+
 @pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
 def test_values_outside_the_counted_range(native, dtype):
     """Logits of 128 and more, of -128 and less that still have a weight, and near zero, also on a border."""

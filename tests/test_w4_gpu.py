@@ -109,6 +109,24 @@ def test_strided_rows_and_untouched_memory(native):
     assert int(flags) == 0
 
 
+def test_offsets_past_32_bits(native):
+    """A weight of 8 GiB, and rows of x further apart than 2^32 bytes."""
+    n, k, group, gen = 1 << 20, 16384, 256, torch.Generator(device=DEV).manual_seed(5)
+    codes = torch.randint(-2 ** 31, 2 ** 31, (n, k // 8), dtype=torch.int32, device=DEV, generator=gen)
+    scales = (0.02 * torch.randn((n, k // group), device=DEV, generator=gen)).to(BF16)
+    bank = native.w4_pack(codes.view(torch.uint32), scales)
+    at = torch.tensor([0, 17, 2 ** 19 - 1, 2 ** 19, 2 ** 19 + 33, n - 300, n - 16, n - 1], device=DEV)
+    c = torch.stack([(codes[at].long() >> (4 * d)) & 15 for d in range(8)], dim=2).view(len(at), k)
+    weight = ((c.view(len(at), -1, group) - 8).double() * scales[at].double()[:, :, None]).view(len(at), k).cpu()
+    del codes
+    stride = 2 ** 31 + 8
+    x = torch.empty(2 * stride + k, dtype=BF16, device=DEV).as_strided((3, k), (stride, 1))
+    x.copy_(rows(3, k, BF16))
+    out, flags = run(native, x, bank, n, FP32)
+    check(out[:, at], x, weight)
+    assert int(flags) == 0
+
+
 def test_extreme_codes_and_scales(native):
     """Codes 0 and 15 against zero points 15 and 0, scales at both ends."""
     n, k = 32, 64
