@@ -16,7 +16,9 @@ so that a caller written for it works unchanged; the code is this library's:
     finite values and scales at or above the 2^-14 floor;
   * `register_packed`, `G256LinearMethod`, `W8HeadMethod` (method.py:11-91):
     packed parameters that accept exactly one copy of their shape and dtype
-    before sealing; apply through `ornith_b200::dense_out` / `head_out`.
+    before sealing; apply through `ornith_b200::dense_out` / `head_out`;
+  * `W4LinearMethod`: the same for a linear layer or a head in the ordinary
+    4-bit checkpoint form, through `ornith_b200::w4_out` (the plugin has none).
 The kernels trust the banks: these admission rules are the only check a
 checkpoint gets.  The layer is any torch.nn.Module (vLLM's layers in the
 reference); rejected loads raise ValueError, as the plugin's do.
