@@ -158,6 +158,23 @@ def test_largest_shares_of_equal_logits(native, vocab):
         check(native, x, u=uniform(150, i), **s)
 
 
+@pytest.mark.parametrize('dtype', [FP16, FP32])
+def test_large_nuclei_of_large_batches(native, dtype):
+    """Nuclei whose border lies among a few thousand tokens of a CTA that are kept apart, among more than it keeps,
+    among equal logits, and below a cut by number."""
+    m, vocab = 150, 40009
+    x = logits_of(m, vocab, FP32, 51)
+    x[1::5] = (x[1::5] * 4).round() / 4            # many equal
+    x[2::5] = 2.0 + x[2::5] / 1000                 # all in one or two bins
+    x[3::5, ::2] = -float('inf')
+    x[4::5] = (x[4::5] > 1.0).float()              # two values
+    x = x.to(dtype)
+    for i, s in enumerate((dict(p=0.9), dict(p=0.5, T=1.7), dict(p=0.99), dict(k=20000, p=0.8), dict(k=9000, p=0.95, T=3.0),
+                           dict(p=0.7, min_p=0.01))):
+        check(native, x, u=uniform(m, 60 + i), **s)
+        check(native, x[:, 1:], u=0.0, **s)
+
+
 def test_rows_further_apart_than_32_bits(native):
     vocab, stride = 70001, 2 ** 31 + 17
     for dtype in (BF16, FP16):
