@@ -35,8 +35,9 @@
 //     by counts that are kept apart for each);
 //   - for fp16 and fp32 the counts bound the masses, and the tokens of the bins
 //     that can hold the border are weighed one by one;
-//   - uncut fp16 and fp32 rows, and those that the counts do not hold (many
-//     tiny values, a largest logit outside +-128), search by bins of value.
+//   - uncut fp16 and fp32 rows are weighed slab by slab, and drawn from;
+//   - rows that the counts do not hold (many tiny values, a largest logit
+//     outside +-128) search a cut by bins of value.
 //
 // What bounds it.  Not HBM (64 uncut fp32 rows of 248320 take 40.0 us, 1.59
 // TB/s): the small cases wait for some ten steps between the CTAs of a row
