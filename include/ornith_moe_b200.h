@@ -522,7 +522,8 @@ ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_w4_launch(
  * -inf logits are never drawn.  A row that cannot be sampled gets token -1 and
  * log probability NaN and raises (sticky) 1: NaN or +inf among its logits,
  * 2: a parameter out of range (temperature outside [0, 1e30], top_p negative,
- * min_p outside [0, 1], uniform outside [0, 1), any NaN), 4: every logit -inf.
+ * min_p outside [0, 1], uniform outside [0, 1), any NaN), 4: every logit -inf,
+ * 128: the kernel found more tokens than it had counted (a defect; none known).
  * 0 <= M, 1 <= vocab <= 524288; type 0 bf16, 1 fp16, 2 fp32; stride: values
  * between rows, at least vocab (unused for one row); any alignment of the
  * type.  temperature, top_p, min_p, uniform fp32 [M], top_k int32 [M]; all but

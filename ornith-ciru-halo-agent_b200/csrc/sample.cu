@@ -79,7 +79,7 @@ constexpr int kParts = 4, kPartVecs = 255 * 32, kMaxVecs = kParts * kPartVecs;
 constexpr int kAloneVecs = 1 << 13, kSharedVecs = 3 << 10;
 constexpr int kStep = 8, kSlabs = kMaxVecs / 32 / kStep + kWarps;  // rows of 32 vectors in a slab; slabs of a CTA
 constexpr float kMaxTemperature = 1e30f;
-constexpr uint32_t kFlagNonfinite = 1, kFlagParameter = 2, kFlagNothingLeft = 4;
+constexpr uint32_t kFlagNonfinite = 1, kFlagParameter = 2, kFlagNothingLeft = 4, kFlagBounds = 128;
 
 struct Args {
     const void* logits;
@@ -976,8 +976,11 @@ __device__ Partition counted_partition(const Row<0>& r) {
     return Partition{as_float(sums.a), as_float(sums.b)};
 }
 
-// Pushes the tokens at `bottom` or above (kList at most) to the cluster's first
-// CTA.  The caller synchronises the cluster next.
+// Pushes the tokens at `bottom` or above to the cluster's first CTA.  The caller
+// synchronises the cluster next, and has made sure that the row has no more than
+// kList of them, by counts that no cut has clipped: every token of the border's
+// value is pushed, also those that top-k leaves out.  (A longer list would have
+// lost tokens: draw_from_list refuses it.)
 template <int TY>
 __device__ void push_list(const Row<TY>& r, float bottom) {
     auto cluster = cg::this_cluster();
@@ -1059,7 +1062,15 @@ template <int TY>
 __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 limit, float p, float u, u64 whole) {
     Shared& sh = shared();
     List& l = sh.values.list;
-    const int tid = threadIdx.x, n = min(int(sh.listed), kList);
+    const int tid = threadIdx.x, n = int(sh.listed);
+    if (n > kList) {
+        if (tid == 0) {
+            a.tokens[row] = -1;
+            if (a.logprobs) a.logprobs[row] = NAN;
+            atomicOr(a.flags, kFlagBounds);
+        }
+        return;
+    }
     Partition z{1.f, 0.f};
     if (a.logprobs) {
         if constexpr (TY == 0)
@@ -1298,9 +1309,12 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
                 if (bin != kTinyBin) sh.bound[1] = ceil_div(target - sh.bound[1], w);
             }
             __syncthreads();
-            border = min(max(sh.found_bin, 0), kValueBins - 1), ties = sh.bound[1];
+            const int nucleus_border = min(max(sh.found_bin, 0), kValueBins - 1);
+            // of top-k's border only a part is in cnt, and more than kList tokens lie at it or above
+            const bool tied = by_count && nucleus_border == border;
+            border = nucleus_border, ties = sh.bound[1];
             if (border == kTinyBin) return false;
-            if (sh.found <= kList) {
+            if (sh.found <= kList && !tied) {
                 push_list(r, near_edge(border));
                 cluster.sync();
                 if (r.rank == 0) draw_from_list(r, a, row, limit, p, u, whole);

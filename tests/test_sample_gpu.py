@@ -385,3 +385,62 @@ def test_hidden_states_to_tokens(native):
     tokens = torch.empty(m, dtype=torch.int32, device=DEV)
     native.sample_out(logits, None, None, None, None, uniform(m, 8).to(DEV), tokens, None, rt.slots[1])
     assert bool(((tokens >= 0) & (tokens < n)).all()) and rt.check_error_flags() == [0, 0]
+
+
+def check_twice(native, x, u, **s):
+    """Against the definition, and the same tokens again."""
+    first, _, _ = run(native, x, u=u, **s)
+    check(native, x, u=u, **s)
+    assert torch.equal(first, run(native, x, u=u, **s)[0])
+
+
+TIED_K, TIED_P = (2, 50, 257, 1000, 1023, 1024), (0.5, 0.9, 0.99, 0.999)
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('vocab', [1500, 70001])
+def test_nucleus_border_among_the_ties_of_a_short_top_k(native, dtype, vocab):
+    """The k-th logit has more equals than a list holds, and the nucleus ends among them: by index, in every call."""
+    x = torch.empty((5, vocab))
+    x[0] = 0.25                                                           # one value
+    x[1] = torch.where(torch.arange(vocab) % 7 == 3, 1.0, 0.5)            # two
+    x[2] = 0.5
+    x[2, vocab // 3::2] = -math.inf
+    x[2, vocab // 2:vocab // 2 + 40] = torch.linspace(1.0, 3.0, 40)       # a few larger logits above the equal ones
+    x[3] = (torch.randn(vocab, generator=torch.Generator().manual_seed(3)) * 40).round() / 40 / 2   # a few hundred
+    x[4] = -0.75
+    x[4, ::2] = -1.0
+    x = x.to(dtype).to(DEV)
+    for i, k in enumerate(TIED_K):
+        for j, p in enumerate(TIED_P):
+            check_twice(native, x, uniform(5, 10 * i + j), k=k, p=p, T=(1.0, 0.7, 3.0)[(i + j) % 3])
+
+
+@pytest.mark.parametrize('m', [1, 3, 150])
+def test_nucleus_border_among_the_ties_of_real_rows(native, m):
+    """Ordinary bf16 rows: flat ones, and ones around 20 whose neighbours lie 1/8 apart."""
+    vocab = 248320
+    x = logits_of(3, vocab, BF16, 71)
+    x[1] = (x[1].float() + 12.0).to(BF16)
+    x[2] = (x[2].float() * 0.5 + 20.0).to(BF16)
+    x = x[torch.arange(m) % 3].contiguous()
+    for i, (k, p) in enumerate(((1000, 0.95), (1000, 0.99), (1024, 0.95), (1024, 0.99), (1023, 0.999), (1024, 0.99999))):
+        u = uniform(3, 80 + i)[torch.arange(m) % 3]
+        if m <= 3:
+            check_twice(native, x, u, k=k, p=p)
+        else:                                # every copy of a row as it is alone
+            many, logp, flags = run(native, x, k=k, p=p, u=u)
+            few, few_logp, _ = run(native, x[:3], k=k, p=p, u=u[:3])
+            assert torch.equal(many, few[torch.arange(m) % 3]) and int(flags) == 0
+
+
+def test_tied_rows_alone_and_among_many(native):
+    for value, dtype in ((0.25, BF16), (20.0, BF16), (-3.0, FP16)):
+        row = torch.full((1, 5000), value, dtype=dtype, device=DEV)
+        many = row.expand(200, -1).contiguous()
+        for k, p in ((50, 0.9), (1024, 0.5), (1000, 0.999)):
+            u = float(uniform(1, k))
+            one, _, _ = run(native, row, k=k, p=p, u=u)
+            kept = math.ceil(float(np.float32(p)) * k)
+            assert int(one) == int(kept * u)                     # equal weights: indices 0 .. kept - 1
+            assert bool((run(native, many, k=k, p=p, u=u)[0] == one).all())
