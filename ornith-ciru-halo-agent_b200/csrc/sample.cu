@@ -645,9 +645,9 @@ __device__ bool cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
     Search& f = sh.search;
     auto cluster = cg::this_cluster();
     const int per = kBins / r.size;  // bins that one CTA merges
-    float scale = 0.f;               // of the last histogram
+    float scale = 0.f, lift = 1.f;   // of the last histogram
     int border = -1;                 // its bin, where there was one
-    auto bin = [&](float x) { return max(0, min(kBins - 1, __float2int_rz(__fmul_rn(__fsub_rn(hi, x), scale)))); };
+    auto bin = [&](float x) { return max(0, min(kBins - 1, __float2int_rz(__fmul_rn(__fmul_rn(__fsub_rn(hi, x), lift), scale)))); };
     // Few logits lie in the range once it is narrow: one branch for the others.
     auto inside = [&](float x, int slot) {
         return (x >= lo & x <= hi) && r.kept(x, slot) && (border < 0 || bin(x) == border);
@@ -660,7 +660,10 @@ __device__ bool cut_row(Row<TY>& r, float lo, float hi, u64 base, u64 target, u6
     };
     while (n > u64(kCap)) {
         border = -1;
-        scale = __fdiv_rn(float(kBins), __fsub_rn(hi, lo));
+        // A range below 2^-118 has no scale in fp32: it would go to the two ends of the histogram, and a round would
+        // take one value off it.
+        lift = __fsub_rn(hi, lo) < 0x1p-64f ? 0x1p80f : 1.f;
+        scale = __fdiv_rn(float(kBins), __fmul_rn(__fsub_rn(hi, lo), lift));
         for (int b = threadIdx.x; b < kBins; b += kThreads) {
             f.cnt[b] = f.tcnt[b] = 0;
             if (MASS) f.mass[b] = f.tmass[b] = 0;

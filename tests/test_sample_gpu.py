@@ -444,3 +444,26 @@ def test_tied_rows_alone_and_among_many(native):
             kept = math.ceil(float(np.float32(p)) * k)
             assert int(one) == int(kept * u)                     # equal weights: indices 0 .. kept - 1
             assert bool((run(native, many, k=k, p=p, u=u)[0] == one).all())
+
+
+def test_logits_a_step_of_the_smallest_number_apart(native):
+    """Thousands of different logits inside a range that has no reciprocal in fp32: each round of the search has to
+    leave a share of them, not all but one."""
+    def steps(vocab, seed):
+        order = torch.randperm(vocab, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        return order.view(FP32).to(DEV)[None]                    # 0, 1, 2 ... times 2^-149
+
+    x = torch.cat([steps(20011, 1), -steps(20011, 2), steps(20011, 3)])
+    x[2, ::3] *= -1
+    for i, s in enumerate((dict(k=9000), dict(p=0.5), dict(k=15000, p=0.3), dict(T=2.0 ** -137, p=0.7), dict(T=2.0 ** -137, k=5000))):
+        check(native, x, u=uniform(3, 90 + i), **s)
+    large, u = steps(1 << 19, 4), 0.625
+    run(native, x, k=9000)                                       # the kernel is loaded
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    token, _, _ = run(native, large, k=1 << 18, u=u)
+    end.record()
+    end.synchronize()
+    kept = torch.arange(1 << 19, device=DEV)[large[0].view(torch.int32) >= 1 << 18]
+    assert int(token) == int(kept[int(u * (1 << 18))])           # equal weights, in order of the indices
+    assert begin.elapsed_time(end) < 100                         # some 0.2 ms; one value a round would take seconds
