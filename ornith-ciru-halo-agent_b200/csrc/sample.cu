@@ -194,6 +194,7 @@ struct Values {
     float tiny[kTinyCap];                          // this CTA's tiny logits (bf16 rows)
     uint8_t tiny_part[kTinyCap];                   // and where they lie
     u64 tiny_mass[kMaxCluster];                    // pushed
+    u64 tiny_sum[kMaxCluster];                     // pushed: of exp(x), times 2^50
 };
 
 // A bin's largest and smallest value; the same for bf16 but in the tiny one.
@@ -961,15 +962,21 @@ __device__ Partition joined_partition(const Row<TY>& r) {
     return z;
 }
 
-// The same in a bf16 row's counts, for a block.
+// The same in a bf16 row's counts, for a block.  The tiny bin's values are not
+// alike (by up to two per mille in their exponentials): theirs are summed apart.
 __device__ Partition counted_partition(const Row<0>& r) {
     const Values& h = shared().values;
     float others = 0.f, tops = 0.f;
+    if (threadIdx.x == kTinyBin / kPerThread && h.all[kTinyBin]) {
+        u64 tiny = 0;
+        for (int q = 0; q < r.size; ++q) tiny += h.tiny_sum[q];
+        others = float(double(tiny) * 0x1p-50 * exp(-double(r.top)));
+    }
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
         const int bin = int(threadIdx.x) * kPerThread + i;
         const float c = float(h.all[bin]);
-        if (c > 0.f) {
+        if (c > 0.f && bin != kTinyBin) {
             const float v = near_edge(bin), e = expf(__fsub_rn(v, r.top));
             tops = v == r.top ? c : tops;
             others = v == r.top ? others : __fmaf_rn(c, e, others);
@@ -1159,11 +1166,12 @@ __device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, float
                                      : Partition{1.f, 0.f});
 }
 
-// The row's counts, by value, in every CTA; and for bf16 the mass of the tiny.
+// The row's counts, by value, in every CTA; and for bf16 the mass of the tiny,
+// with `logprobs` the sum of their exponentials too (integers: in any order).
 // Each CTA adds up a range of codes, four at a time, in its own copy of the
 // result, and pushes that to the others.
 template <int TY>
-__device__ u64 merge_counts(const Row<TY>& r, uint32_t tiny_count) {
+__device__ u64 merge_counts(const Row<TY>& r, uint32_t tiny_count, bool logprobs) {
     Values& h = shared().values;
     auto cluster = cg::this_cluster();
     const int tid = threadIdx.x, quads = 2 * kCodes / 4 / r.size, first = r.rank * quads;
@@ -1201,15 +1209,19 @@ __device__ u64 merge_counts(const Row<TY>& r, uint32_t tiny_count) {
         const int tiny = int(h.own[2 * kCodes]);
         if ((tid & ~31) < tiny) {  // whole warps
             u64 w = tid < tiny ? r.weight(h.tiny[tid]) : 0;
+            u64 e = tid < tiny && logprobs ? __double2ull_rn(exp(double(h.tiny[tid])) * 0x1p50) : 0;
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
-            if ((tid & 31) == 0) atomicAdd(&shared().bound[0], w);  // integers: in any order
+            for (int d = 16; d > 0; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d), e += __shfl_xor_sync(0xffffffffu, e, d);
+            if ((tid & 31) == 0) atomicAdd(&shared().bound[0], w), atomicAdd(&shared().bound[1], e);
         }
     }
     __syncthreads();
     if (TY == 0) {
         own_tiny = shared().bound[0];
-        if (tid < r.size) *cluster.map_shared_rank(&h.tiny_mass[r.rank], tid) = own_tiny;
+        if (tid < r.size) {
+            *cluster.map_shared_rank(&h.tiny_mass[r.rank], tid) = own_tiny;
+            *cluster.map_shared_rank(&h.tiny_sum[r.rank], tid) = shared().bound[1];
+        }
     }
     for (int i = tid; i < quads * (r.size - 1); i += kThreads) {
         const int to = (r.rank + 1 + i / quads) & (r.size - 1), at = place(first + i % quads);
@@ -1229,7 +1241,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
     Values& h = sh.values;
     auto cluster = cg::this_cluster();
     const int tid = threadIdx.x;
-    const u64 own_tiny = merge_counts(r, tiny_count);
+    const u64 own_tiny = merge_counts(r, tiny_count, a.logprobs);
     const u64 limit = greedy ? 1 : k > 0 && k < a.vocab ? u64(k) : ~u64(0);
     if (greedy) p = 1.f;
 
@@ -1638,7 +1650,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     if (TY == 0 && a.part_vecs)
         for (int i = tid; i < kCodes; i += kThreads) vectors()[i] = make_uint4(0, 0, 0, 0);  // kParts / 2 * 2 * kCodes words
     if (tid < 256) sh.pow256[tid] = exp2(frac - tid * (1.0 / 256));
-    if (tid == 0) sh.listed = 0, sh.bound[0] = 0;
+    if (tid == 0) sh.listed = 0, sh.bound[0] = sh.bound[1] = 0;
     __syncthreads();
     float top = -INFINITY;
     bool strange = false;

@@ -467,3 +467,20 @@ def test_logits_a_step_of_the_smallest_number_apart(native):
     kept = torch.arange(1 << 19, device=DEV)[large[0].view(torch.int32) >= 1 << 18]
     assert int(token) == int(kept[int(u * (1 << 18))])           # equal weights, in order of the indices
     assert begin.elapsed_time(end) < 100                         # some 0.2 ms; one value a round would take seconds
+
+
+@pytest.mark.parametrize('vocab', [300, 1003, 9001, 50257])
+def test_log_probability_beside_many_tiny_logits(native, vocab):
+    """bf16 logits below 2^-10 share a count, but not an exponential: their sum is the model's all the same."""
+    gen = torch.Generator().manual_seed(vocab)
+    x = torch.full((6, vocab), -9.0)
+    few = min(250, vocab - 20)
+    x[:, :few] = 9.6e-4                                            # all on one side of zero
+    x[1, :few] = -9.6e-4
+    x[2, :few] = (torch.rand(few, generator=gen) * 2 - 1) * 9.7e-4
+    x[3, :few // 2] = 0.0
+    x[4:, :few] = torch.rand((2, few), generator=gen) * 9.7e-4
+    x[:, few + 3] = torch.tensor([0.01, 0.01, 0.002, 1.0, 3.0, 0.5])
+    x = x[:, torch.randperm(vocab, generator=gen)].to(BF16).to(DEV)
+    for i, s in enumerate((dict(), dict(T=0.7), dict(k=20), dict(p=0.9), dict(k=700, p=0.99), dict(T=0.0), dict(min_p=0.99))):
+        check(native, x, u=uniform(6, 110 + i), **s)
