@@ -232,7 +232,7 @@ struct alignas(16) Shared {
     Pair slot[2][kMaxCluster];           // pushed by every CTA of the cluster in turn
     u64 slab[kSlabs];                    // kept mass of each slab, in index order
     Pair red[kWarps];
-    Pair part[kMaxCluster];              // fp16, fp32: every CTA's largest logit, count of it and sum of the others
+    Pair part[kMaxCluster];              // fp16, fp32: every CTA's largest logit, sum of exponentials against it
     u64 bound[2];
     uint32_t part_here[kParts], part_kept[kParts];  // the border's value in the parts of the token's CTA
     int found, found_bin;
@@ -279,6 +279,22 @@ __device__ __noinline__ uint4 edge_vector(const char* begin, int i0, int vocab) 
         }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// 2^s exp(-d / T) for d >= 0, with step = 256 log2(e) / T; no more than 600 T.
+__device__ __forceinline__ double scaled_exp(double d, double step) {
+    constexpr double a = 0.69314718055994530942 / 256, kRound = 0x1.8p52;
+    const double shifted = __fma_rn(d, step, kRound);  // n = rint(256 d log2(e) / T) in its low bits
+    const int n = __double2loint(shifted);
+    const double f = __fma_rn(d, step, -__dsub_rn(shifted, kRound));
+    double p = __fma_rn(f, -a * a * a / 6, a * a / 2);
+    p = __fma_rn(p, f, -a);
+    p = __fma_rn(p, f, 1.0);
+    const double v = __dmul_rn(shared().pow256[n & 255], p);
+    return __hiloint2double(__double2hiint(v) + (n & ~255) * -4096, __double2loint(v));  // times 2^-(n / 256)
+}
+constexpr double kStep1 = 256 * 1.4426950408889634074;  // at T = 1
+// 2^-s
+__device__ __forceinline__ double unit() { return __hiloint2double((2046 << 20) - __double2hiint(shared().pow256[0]), 0); }
 
 // What every thread of a row's cluster knows.
 template <int TY>
@@ -347,17 +363,9 @@ struct Row {
 
     // 2^52 + the fixed-point weight, as the bits of a double; 2^52 where not `in`.
     __device__ __forceinline__ u64 raw_weight(float x, bool in) const {
-        constexpr double a = 0.69314718055994530942 / 256, kRound = 0x1.8p52;
-        const double d = __dsub_rn(double(top), double(x));
-        const double shifted = __fma_rn(d, step, kRound);  // n = rint(256 d log2(e) / T) in its low bits
-        const int n = __double2loint(shifted);
-        const double f = __fma_rn(d, step, -__dsub_rn(shifted, kRound));
-        double p = __fma_rn(f, -a * a * a / 6, a * a / 2);
-        p = __fma_rn(p, f, -a);
-        p = __fma_rn(p, f, 1.0);
-        const double v = __dmul_rn(shared().pow256[n & 255], p);
-        const int high = __double2hiint(v) + (n & ~255) * -4096;  // times 2^-(n / 256)
-        return u64(__double_as_longlong(__dadd_rn(__hiloint2double(in ? high : 0, __double2loint(v)), 0x1p52)));
+        const double v = scaled_exp(__dsub_rn(double(top), double(x)), step);
+        const int high = in ? __double2hiint(v) : 0;
+        return u64(__double_as_longlong(__dadd_rn(__hiloint2double(high, __double2loint(v)), 0x1p52)));
     }
     static constexpr u64 kRawZero = 0x4330000000000000ull;
     __device__ __forceinline__ u64 weight(float x) const {
@@ -891,44 +899,58 @@ __device__ u64 slab_masses(const Row<TY>& r, const Region& g) {
     return mine;
 }
 
-// The log probability of a token x: sums of exp(logit - top) over the largest
-// logits (`tops` of them) and the others.
-struct Partition {
-    float tops, others;
-    __device__ float of(float x, float top) const {
-        return float((double(x) - double(top)) - double(__fadd_rn(logf(tops), log1pf(__fdiv_rn(others, tops)))));
-    }
-};
+// The log probability of a token x: `sum` is that of exp(logit - top) over all
+// tokens, 1 at least and 2^19 at most.  In 64 bits up to here, rounded once: the
+// logarithm is an fp32 one put right by a Newton step, whose remainder is below
+// 1e-12 (a chain of a third of a double-precision logarithm's steps, in which
+// every row waits for one thread).
+__device__ __forceinline__ float log_probability(float x, float top, double sum) {
+    const float guess = logf(float(sum));
+    const double rest = __fma_rn(__dmul_rn(sum, unit()), scaled_exp(double(guess), kStep1), -1.0);
+    return float((double(x) - double(top)) - double(guess) - rest);
+}
 
 // For the CTA that holds the token.
 template <int TY>
-__device__ void write_token(const Row<TY>& r, const Args& a, int row, u64 ahead, u64 target, const Partition& z) {
+__device__ void write_token(const Row<TY>& r, const Args& a, int row, u64 ahead, u64 target, double z) {
     find_value(r, ahead, target, [&](float x, int slot) { return r.kept(x, slot) ? r.weight(x) : 0; },
                [&](float x, int slot) {
                    a.tokens[row] = r.first + slot;
-                   if (a.logprobs) a.logprobs[row] = z.of(x, r.top);
+                   if (a.logprobs) a.logprobs[row] = log_probability(x, r.top, z);
                });
 }
 
-__device__ __forceinline__ Pair add_floats(Pair p, Pair q) {
-    return Pair{as_bits(__fadd_rn(as_float(p.a), as_float(q.a))), as_bits(__fadd_rn(as_float(p.b), as_float(q.b)))};
-}
-// This CTA's logits equal to `top`, counted, and the others' exp(x - top),
-// summed: vector by vector, so that no sum has more than some 70 steps.
+__device__ __forceinline__ double as_double(u64 v) { return __longlong_as_double(static_cast<long long>(v)); }
+__device__ __forceinline__ u64 as_bits(double v) { return u64(__double_as_longlong(v)); }
+__device__ __forceinline__ Pair add_doubles(Pair p, Pair q) { return Pair{as_bits(as_double(p.a) + as_double(q.a)), 0}; }
+
+// The sum of exp(x - top) over this CTA's logits.  Those up to kReach below `top`
+// are taken in 64 bits: for fp16 and fp32 they are few, and a row's sum can rest
+// on one of them.  The others go through fp32 one vector at a time, each off by
+// at most (|x - top| + 4) steps of 2^-24 of itself and 7 of its vector's sum;
+// they have e^-2 at most each, so what is left of these steps averages out.
+// Vectors are joined in 64 bits.  64 flat fp32 rows of 248320 at T = 0.7: 60.7 us
+// in all, 64.9 where the fp32 ones start at 3, 78 with all in 64 bits, and 59.4
+// with all in fp32.
 template <int TY>
-__device__ Pair exponentials(const Row<TY>& r, float top) {
-    float equal = 0.f, others = 0.f;
+__device__ double exponentials(const Row<TY>& r, float top) {
+    constexpr int E = Elem<TY>::E;
+    double sum = 0.0, close = 0.0;
+    constexpr float kReach = TY == 0 ? 600.f : 2.f;
+    const float near = __fsub_rn(top, kReach);
     r.each_vector([&](int, const uint4& q) {
-        float x[Elem<TY>::E], sum = 0.f;
+        float x[E], part = 0.f;
         Elem<TY>::unpack(q, x);
 #pragma unroll
-        for (int e = 0; e < Elem<TY>::E; ++e) {
-            equal += x[e] == top ? 1.f : 0.f;
-            sum += x[e] == top ? 0.f : expf(__fsub_rn(x[e], top));
+        for (int e = 0; e < E; ++e) part += x[e] >= near ? 0.f : expf(__fsub_rn(x[e], top));
+        sum += double(part);
+        if (Elem<TY>::largest(q) >= near) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (x[e] >= near) close += scaled_exp(double(top) - double(x[e]), kStep1);
         }
-        others += sum;
     });
-    return block_reduce(Pair{as_bits(equal), as_bits(others)}, add_floats);
+    return as_double(block_reduce(Pair{as_bits(__fma_rn(close, unit(), sum)), 0}, add_doubles).a);
 }
 __device__ __forceinline__ Pair add_pairs(Pair p, Pair q) { return Pair{p.a + q.a, p.b + q.b}; }
 
@@ -940,50 +962,40 @@ __device__ __forceinline__ u64 nucleus(u64 mass, float p) {
     return max(u64(1), __umul64hi(mass, share) + (mass * share != 0));
 }
 
-// The largest logits of a row and the others, from what every CTA has of them.
-// For a warp: every lane gets it.
+// The sum of a row's exponentials from what every CTA has of it.  For a warp:
+// every lane gets it.
 template <int TY>
-__device__ Partition joined_partition(const Row<TY>& r) {
-    Partition z{0.f, 0.f};
+__device__ double joined_partition(const Row<TY>& r) {
+    double z = 0.0;
     const int lane = threadIdx.x & 31;
     if (lane < r.size) {
         const Pair part = shared().part[lane];
-        const float local = as_float(part.a), equal = as_float(part.b), others = as_float(part.b >> 32);
-        if (local == r.top)
-            z = Partition{equal, others};
-        else if (local > -INFINITY)
-            z.others = __fmul_rn(__fadd_rn(equal, others), expf(__fsub_rn(local, r.top)));
+        const float local = as_float(part.a);
+        if (local >= r.top - 600.f) z = as_double(part.b) * (scaled_exp(double(r.top) - double(local), kStep1) * unit());
     }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        z.tops += __shfl_xor_sync(0xffffffffu, z.tops, d);
-        z.others += __shfl_xor_sync(0xffffffffu, z.others, d);
-    }
+    for (int d = 16; d > 0; d >>= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
     return z;
 }
 
-// The same in a bf16 row's counts, for a block.  The tiny bin's values are not
+// The same from a bf16 row's counts, for a block.  The tiny bin's values are not
 // alike (by up to two per mille in their exponentials): theirs are summed apart.
-__device__ Partition counted_partition(const Row<0>& r) {
+__device__ double counted_partition(const Row<0>& r) {
     const Values& h = shared().values;
-    float others = 0.f, tops = 0.f;
-    if (threadIdx.x == kTinyBin / kPerThread && h.all[kTinyBin]) {
-        u64 tiny = 0;
-        for (int q = 0; q < r.size; ++q) tiny += h.tiny_sum[q];
-        others = float(double(tiny) * 0x1p-50 * exp(-double(r.top)));
-    }
-#pragma unroll
+    double sum = 0.0;
+#pragma unroll 3
     for (int i = 0; i < kPerThread; ++i) {
         const int bin = int(threadIdx.x) * kPerThread + i;
-        const float c = float(h.all[bin]);
-        if (c > 0.f && bin != kTinyBin) {
-            const float v = near_edge(bin), e = expf(__fsub_rn(v, r.top));
-            tops = v == r.top ? c : tops;
-            others = v == r.top ? others : __fmaf_rn(c, e, others);
-        }
+        const uint32_t c = h.all[bin];
+        if (c && bin != kTinyBin) sum = __fma_rn(double(c), scaled_exp(double(r.top) - double(near_edge(bin)), kStep1), sum);
     }
-    const Pair sums = block_reduce(Pair{as_bits(tops), as_bits(others)}, add_floats);
-    return Partition{as_float(sums.a), as_float(sums.b)};
+    sum *= unit();
+    if (threadIdx.x == 0 && h.all[kTinyBin]) {
+        u64 tiny = 0;
+        for (int q = 0; q < r.size; ++q) tiny += h.tiny_sum[q];
+        sum += double(tiny) * 0x1p-50 * exp(-double(r.top));
+    }
+    return as_double(block_reduce(Pair{as_bits(sum), 0}, add_doubles).a);
 }
 
 // Pushes the tokens at `bottom` or above to the cluster's first CTA.  The caller
@@ -1081,7 +1093,7 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
         }
         return;
     }
-    Partition z{1.f, 0.f};
+    double z = 1.0;
     if (a.logprobs) {
         if constexpr (TY == 0)
             z = counted_partition(r);
@@ -1106,7 +1118,7 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
     const u64 target = drawn(mass, u);
     const auto answer = [&](int rank) {
         a.tokens[row] = l.i[rank];
-        if (a.logprobs) a.logprobs[row] = z.of(l.v[rank], r.top);
+        if (a.logprobs) a.logprobs[row] = log_probability(l.v[rank], r.top, z);
     };
     if (keep <= kThreads / 2) {
         // mass up to each kept token in index order, by two threads
@@ -1147,10 +1159,11 @@ __device__ void draw_from_list(const Row<TY>& r, const Args& a, int row, u64 lim
     }
 }
 
-// Kept masses of the CTAs -> the one that holds the token finds it.  unit: where
-// that mass times it is the sum of exponentials for the log probability; else 0.
+// Kept masses of the CTAs -> the one that holds the token finds it.  from_mass:
+// that mass is the sum of exponentials for the log probability too (off by half a
+// unit of 2^-s a token at most, so by 2^-27 in all for 2^18 tokens).
 template <int TY>
-__device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, float unit, const Region* g = nullptr) {
+__device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, bool from_mass, const Region* g = nullptr) {
     const Pair own = block_reduce(Pair{g ? slab_masses(r, *g) : slab_masses(r), 0}, add_pairs);
     const Pair* all = r.exchange(own);
     u64 whole = 0, ahead = 0;
@@ -1161,9 +1174,7 @@ __device__ void draw_from_row(Row<TY>& r, const Args& a, int row, float u, float
     const u64 target = drawn(whole, u);
     if (ahead <= target && target < ahead + own.a)
         write_token(r, a, row, ahead, target,
-                    unit != 0.f      ? Partition{1.f, float(double(whole) * unit - 1.0)}
-                    : a.logprobs ? joined_partition(r)
-                                     : Partition{1.f, 0.f});
+                    !a.logprobs ? 1.0 : from_mass ? double(whole) * unit() : joined_partition(r));
 }
 
 // The row's counts, by value, in every CTA; and for bf16 the mass of the tiny,
@@ -1364,8 +1375,7 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
         const u64 target = drawn(whole, u);
         if (ahead > target || target >= ahead + own.a) return true;
         // the CTA that holds the token
-        Partition z{1.f, 0.f};
-        if (a.logprobs) z = counted_partition(r);
+        const double z = a.logprobs ? counted_partition(r) : 1.0;
         u64 target_at = ahead;
         if (a.part_vecs) {
             // the part that holds it, by the parts' counts
@@ -1485,12 +1495,12 @@ __device__ bool counted_row(Row<TY>& r, const Args& a, int row, int k, float p, 
             const Region* g = keep && proved && region().n <= uint32_t(kRegion) ? &region() : nullptr;
             const bool cut = cut_row<TY, true>(r, low_enough ? bottom : r.weigh_from, high_enough ? edge : r.top, high_enough ? base : 0,
                                                target, proved ? counts_close - counts_open : a.vocab, g);
-            draw_from_row(r, a, row, u, 0.f, cut ? g : nullptr);
+            draw_from_row(r, a, row, u, false, cut ? g : nullptr);
             return true;
         } else if (by_count) {
             cut_row<TY, false>(r, fmaxf(bin_bottom(border), floor_v), bin_top(border), before, limit, listed - before);
         }
-        draw_from_row(r, a, row, u, 0.f);
+        draw_from_row(r, a, row, u, false);
         return true;
     }
 }
@@ -1703,14 +1713,11 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
     // Uncut at T = 1, the weights are those exponentials (fp16, fp32; the counts of bf16 give them anyhow).
     const bool from_mass = TY != 0 && a.logprobs && T == 1.f && !cuts && min_p == 0.f && u != 0.f;
     // sum of exponentials for the log probability, against this CTA's largest logit; a bf16 row takes it from its counts
-    Pair sums{0, 0};
-    if (TY != 0 && a.logprobs && !from_mass) {
-        const float local = as_float(mine.a);
-        sums = exponentials(r, local);
-    }
+    double sum = 0.0;
+    if (TY != 0 && a.logprobs && !from_mass) sum = exponentials(r, as_float(mine.a));
     cluster.barrier_wait();
     const uint32_t own_tiny = counting ? h.own[2 * kCodes] : 0;
-    const Pair* all = r.exchange(Pair{mine.a | (mine.b | own_tiny << 8) << 32, sums.a | sums.b << 32});
+    const Pair* all = r.exchange(Pair{mine.a | (mine.b | own_tiny << 8) << 32, as_bits(sum)});
     uint32_t tiny_count = 0;
     top = -INFINITY, notes = 0;
     for (int i = 0; i < size; ++i) {
@@ -1745,8 +1752,8 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
 
     // The general way: rows without a cut, and those that the counts do not tell enough about.
     if (TY == 0 && a.logprobs) {
-        const Pair own = exponentials(r, top);
-        if (tid < size) *cluster.map_shared_rank(&sh.part[rank], tid) = Pair{as_bits(top), own.a | own.b << 32};
+        const double own = exponentials(r, top);
+        if (tid < size) *cluster.map_shared_rank(&sh.part[rank], tid) = Pair{as_bits(top), as_bits(own)};
         cluster.sync();
     }
     const bool by_count = greedy || (k > 0 && k < a.vocab), by_mass = p < 1.f && !greedy;
@@ -1777,7 +1784,7 @@ __global__ __launch_bounds__(kThreads, 2) void sample_kernel(const Args a) {
             r.weigh(counted, frac, T);
         }
     }
-    draw_from_row(r, a, row, u, from_mass ? 1.f / float(1ull << frac) : 0.f);
+    draw_from_row(r, a, row, u, from_mass);
 }
 
 std::atomic<bool> g_attr[3][64];

@@ -484,3 +484,39 @@ def test_log_probability_beside_many_tiny_logits(native, vocab):
     x = x[:, torch.randperm(vocab, generator=gen)].to(BF16).to(DEV)
     for i, s in enumerate((dict(), dict(T=0.7), dict(k=20), dict(p=0.9), dict(k=700, p=0.99), dict(T=0.0), dict(min_p=0.99))):
         check(native, x, u=uniform(6, 110 + i), **s)
+
+
+def check_logprob(native, x, u, **s):
+    """A log probability is computed in 64 bits and rounded once: half a step of its own, 2^-24 relative.  Beside that
+    (a) exponentials from a table and the logarithm are off by 1e-12; (b) the sum of an uncut fp16 or fp32 row at T = 1 is that
+    of weights in units of 2^-s, each off by half of one; (c) other fp16 and fp32 rows take the logits of more than 2
+    below their CTA's largest through fp32: off by 2^-24 for each unit of the difference, 4 times that for the
+    exponential and 7 for a vector's sum, each of the logit's own share."""
+    tokens, logp, _ = run(native, x, u=u, **s)
+    x64 = x.double().cpu()
+    vocab = x.shape[1]
+    diff = x64 - x64.max(1, keepdim=True).values
+    e = diff.exp()
+    at = tokens.long().cpu()[:, None]
+    assert bool((at >= 0).all())
+    others = torch.where(torch.arange(vocab)[None] == at, 0.0, (x64 - x64.gather(1, at)).exp()).sum(1)
+    want = -torch.log1p(others)
+    slack = torch.full_like(want, 1e-12)
+    if x.dtype != BF16:
+        slack += vocab * 2.0 ** -(min(51, 62 - (vocab - 1).bit_length()) + 1)
+        if s:
+            slack += (torch.where(diff < -2, e * (11 - diff.clamp_min(-100)), 0.0).sum(1) / e.sum(1)) * 2.0 ** -24
+    err = (logp.double().cpu() - want).abs()
+    tol = 2.0 ** -24 * want.abs() + slack
+    assert bool((err <= tol).all()), f'off by {float((err / tol).max()):.3g} of the bound'
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('m,vocab', [(60, 700), (24, 4099), (40, 50257), (8, 248320)])
+def test_log_probability_to_half_a_step(native, dtype, m, vocab):
+    for i, s in enumerate((dict(), dict(T=0.7), dict(p=0.9), dict(T=1.4, k=50, p=0.95), dict(T=0.0), dict(min_p=0.05),
+                           dict(k=3000), dict(T=2.0))):
+        x = logits_of(m, vocab, dtype, 120 + i, spread=(2.0, 5.0)[i % 2], head=min(vocab // 4, 64))
+        check_logprob(native, x, uniform(m, 130 + i), **s)
+    if dtype is BF16:                                        # the way of rows that the counts do not hold
+        check_logprob(native, (x.float() + 130.0).to(BF16), uniform(m, 140))
