@@ -246,6 +246,8 @@ class W4LinearMethod(G256LinearMethod):
                         attrs.get('device'))
 
     def process_weights_after_loading(self, layer):
+        if layer._g256_ready:   # sealed: the checkpoint form is gone
+            return
         super().process_weights_after_loading(layer)
         layer._g256_ready = False
         checkpoint = [getattr(layer, name).data for name in self.fields]

@@ -95,3 +95,28 @@ def test_method_geometry_and_loading():
             layer.w4_scales.weight_loader(layer.w4_scales, torch.ones((48, 4)))   # another dtype
         with pytest.raises(RuntimeError):
             m.apply(layer, torch.zeros((1, 256), dtype=torch.bfloat16))
+
+
+def test_sealing_twice_and_after_a_refusal(monkeypatch):
+    """A second call of process_weights_after_loading leaves a sealed layer as it is (as for the G256 methods); a
+    weight that the layout refuses leaves the layer unsealed and its parameters in place."""
+    method = importlib.import_module('ornith_b200.method')
+    layer = torch.nn.Module()
+    m = method.W4LinearMethod('layer', group=64)
+    m.create_weights(layer, 256, [48], 256, 48, torch.bfloat16)
+    layer.w4_codes.weight_loader(layer.w4_codes, torch.zeros((48, 32), dtype=torch.uint32))
+    layer.w4_scales.weight_loader(layer.w4_scales, torch.ones((48, 4), dtype=torch.bfloat16))
+
+    def refuse(*checkpoint):
+        raise ValueError('scales must be finite')
+
+    monkeypatch.setattr(method.native, 'w4_pack', refuse)
+    with pytest.raises(ValueError):
+        m.process_weights_after_loading(layer)
+    assert not layer._g256_ready and hasattr(layer, 'w4_codes')
+    packed = []
+    monkeypatch.setattr(method.native, 'w4_pack', lambda *checkpoint: packed.append(checkpoint) or ('tiles', 'scales', None))
+    m.process_weights_after_loading(layer)
+    assert layer._g256_ready and not hasattr(layer, 'w4_codes')
+    m.process_weights_after_loading(layer)
+    assert layer._g256_ready and layer.w4_bank == ('tiles', 'scales', None) and len(packed) == 1
