@@ -520,3 +520,40 @@ def test_log_probability_to_half_a_step(native, dtype, m, vocab):
         check_logprob(native, x, uniform(m, 130 + i), **s)
     if dtype is BF16:                                        # the way of rows that the counts do not hold
         check_logprob(native, (x.float() + 130.0).to(BF16), uniform(m, 140))
+
+
+def test_hidden_states_to_tokens_captured(native):
+    """The same step as a server captures it: the head's method and the sampler in one graph, replayed on new rows."""
+    method = importlib.import_module('ornith_b200.method')
+    runtime = importlib.import_module('ornith_b200.runtime')
+    n, k, m = 32000, 2048, 20
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    layer = torch.nn.Module()
+    head = method.W4LinearMethod('head', group=64, logits_fp32=True)
+    head.create_weights(layer, k, [n], k, n, BF16, device=DEV)
+    codes = torch.randint(-2 ** 31, 2 ** 31, (n, k // 8), dtype=torch.int32, device=DEV, generator=gen)
+    layer.w4_codes.weight_loader(layer.w4_codes, codes.view(torch.uint32))
+    layer.w4_scales.weight_loader(layer.w4_scales, (0.01 * torch.rand((n, k // 64), device=DEV, generator=gen)).to(BF16))
+    head.process_weights_after_loading(layer)
+    rt = runtime.Runtime(['head', 'sampler'], 32, DEV)
+    head.bind(rt, 0)
+    x = torch.randn((m, k), device=DEV, generator=gen).to(BF16)
+    T, p, u = torch.full((m,), 0.8, device=DEV), torch.full((m,), 0.95, device=DEV), uniform(m, 1).to(DEV)
+    tokens, logp = torch.empty(m, dtype=torch.int32, device=DEV), torch.empty(m, device=DEV)
+    head.apply(layer, x)                                         # loaded before the capture
+    native.sample_out(head.apply(layer, x), T, None, p, None, u, tokens, logp, rt.slots[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = head.apply(layer, x)
+        native.sample_out(logits, T, None, p, None, u, tokens, logp, rt.slots[1])
+    for seed in (2, 3):
+        x.copy_(torch.randn((m, k), device=DEV, generator=gen).to(BF16))
+        u.copy_(uniform(m, seed))
+        tokens.fill_(-7)
+        graph.replay()
+        eager = head.apply(layer, x)
+        assert torch.equal(logits, eager)
+        want, want_logp, _ = run(native, eager, T=0.8, p=0.95, u=uniform(m, seed))
+        assert torch.equal(tokens, want) and torch.equal(logp, want_logp)
+        check(native, eager, T=0.8, p=0.95, u=uniform(m, seed))
+    assert rt.check_error_flags() == [0, 0]

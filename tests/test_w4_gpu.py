@@ -230,3 +230,32 @@ def test_layer_method(native):
         assert out.shape == (5, 7, n) and out.dtype == (FP32 if fp32 else BF16)
         check(out.view(35, n), x, weight)
     assert rt.check_error_flags() == [0]
+
+
+@pytest.mark.parametrize('group,k', [(32, 96), (64, 192), (128, 256), (256, 512)])
+@pytest.mark.parametrize('zeros,dtype,scale_dtype', [(False, BF16, BF16), (True, FP16, FP16), (True, BF16, FP16),
+                                                     (False, FP16, BF16)])
+def test_two_row_tiles_a_warp(native, group, k, zeros, dtype, scale_dtype):
+    """Weights wide enough for a warp to take two row tiles, the last set with one of its own, ragged."""
+    n = 4736 * 16 + 9
+    codes, scales, z, weight = make(n, k, group, zeros, dtype, scale_dtype)
+    bank = native.w4_pack(codes, scales, z)
+    for m, out_dtype in ((1, FP32), (8, dtype), (9, FP32), (16, dtype)):
+        x = rows(m, k, dtype, seed=m)
+        around = torch.full((m + 2, n), 7.0, dtype=out_dtype, device=DEV)
+        flags = torch.zeros(1, dtype=torch.int32, device=DEV)
+        native.w4_launch(x, *bank, around[1:-1], flags, n, k)
+        check(around[1:-1], x, weight)
+        assert bool((around[0] == 7).all()) and bool((around[-1] == 7).all()) and int(flags) == 0
+
+
+@pytest.mark.parametrize('group', [32, 64, 128])
+def test_two_warps_share_a_row_tile(native, group):
+    n, k = 20000, 256
+    codes, scales, z, weight = make(n, k, group, True)
+    bank = native.w4_pack(codes, scales, z)
+    for m in (1, 9):
+        x = rows(m, k, BF16, seed=m)
+        out, flags = run(native, x, bank, n)
+        check(out, x, weight)
+        assert int(flags) == 0
