@@ -355,10 +355,12 @@ struct Row {
         }
     }
 
-    // By mass, or (count) by number of tokens that have a weight in double precision.
+    // By mass, or (count) by number of tokens that have a weight in double precision: down to half its smallest
+    // number, 2^-1075.
     __device__ void weigh(bool count, int frac, float T) {
         count_mode = count;
-        weigh_from = fmaxf(-FLT_MAX, __double2float_ru(double(top) - (count ? 744.0 : 0.6931471805599453 * (frac + 1)) * double(T)));
+        const double reach = 0.69314718055994530942 * (count ? 1075 : frac + 1);
+        weigh_from = fmaxf(-FLT_MAX, __double2float_ru(double(top) - reach * double(T)));
     }
 
     // 2^52 + the fixed-point weight, as the bits of a double; 2^52 where not `in`.

@@ -557,3 +557,23 @@ def test_hidden_states_to_tokens_captured(native):
         assert torch.equal(tokens, want) and torch.equal(logp, want_logp)
         check(native, eager, T=0.8, p=0.95, u=uniform(m, seed))
     assert rt.check_error_flags() == [0, 0]
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+def test_the_lightest_tokens_of_a_zero_random_number(native, dtype):
+    """u = 0 draws the first kept token that has a weight in 64 bits, down to the smallest."""
+    x = torch.full((4, 700), -10.0)
+    x[:, 500] = 64.0
+    x[0, 2], x[0, 5] = -10.5, -10.0
+    x[1, 2], x[1, 5] = -10.375, 8.0
+    x[2, 2], x[2, 5] = -10.4375, 8.0
+    x[3] = -30.0
+    x[3, 500] = 64.0
+    x = x.to(dtype).to(DEV)
+    x[:, :2] = -math.inf
+    # 2^-1075 is e^-745.133: at T = 0.1 a difference of 74.51, so -10.5 (74.5) has a weight, and -30 (94) none
+    for s in (dict(T=0.1), dict(T=0.1, k=600), dict(T=0.1, p=1.0, min_p=0.0), dict(T=0.1, k=699)):
+        check(native, x, u=0.0, **s)
+        tokens, _, _ = run(native, x, u=0.0, **s)
+        if 'k' not in s:
+            assert tokens.tolist() == [2, 2, 2, 500]
