@@ -1805,7 +1805,8 @@ extern "C" cudaError_t ornith_moe_b200_sample_launch(const void* logits, int64_t
     if (M < 0 || vocab < 1 || vocab > kMaxVocab || type < 0 || type > 2) return cudaErrorInvalidValue;
     if (M == 0) return cudaSuccess;
     if (M == 1) stride = vocab;
-    if (stride < vocab || stride > (int64_t(1) << 40)) return cudaErrorInvalidValue;
+    // the rows' extent in bytes fits 64 bits, so that the checks below see all of it
+    if (stride < vocab || stride > (int64_t(1) << 40) || M > (int64_t(1) << 60) / stride) return cudaErrorInvalidValue;
     const int bytes = type == 2 ? 4 : 2, per_vec = 16 / bytes;
     const size_t rows4 = size_t(M) * 4, row_bytes = (size_t(M - 1) * size_t(stride) + size_t(vocab)) * bytes;
     for (const void* param : {temperature, top_k, top_p, min_p}) {  // each may be null

@@ -38,3 +38,12 @@ def test_python_refuses_cpu_tensors(native):
     with pytest.raises(ValueError):
         native.sample_launch(torch.zeros((2, 16)), None, None, None, None, torch.zeros(2),
                              torch.zeros(2, dtype=torch.int32), None, torch.zeros(1, dtype=torch.int32))
+
+
+def test_rows_that_wrap_the_address_space(native):
+    """Rows times stride beyond 64 bits must not pass for a small tensor."""
+    fn = native.lib().ornith_moe_b200_sample_launch
+    at = [C.c_void_p((1 << 30) + (i << 32)) for i in range(9)]
+    for m, stride, type_ in (((1 << 24) + 1, 1 << 40, 0), ((1 << 22) + 1, 1 << 40, 2), ((1 << 30) + 1, 1 << 33, 1),
+                             ((1 << 31) - 1, 1 << 40, 2)):
+        assert fn(at[0], stride, type_, *at[1:], m, 1000, None) == INVALID, (m, stride)
