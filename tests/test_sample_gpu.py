@@ -577,3 +577,48 @@ def test_the_lightest_tokens_of_a_zero_random_number(native, dtype):
         tokens, _, _ = run(native, x, u=0.0, **s)
         if 'k' not in s:
             assert tokens.tolist() == [2, 2, 2, 500]
+
+
+def test_two_streams_and_one_flag_word(native):
+    """Calls that overlap on two streams share nothing but the flag word they are given."""
+    x = [logits_of(6, 50257, dtype, 150 + i, head=40) for i, dtype in enumerate((BF16, FP32))]
+    x[1][4, 17] = math.nan
+    u = uniform(6, 9).to(DEV)
+    p = torch.full((6,), 0.9, device=DEV)
+    want = [run(native, v, p=p, u=u) for v in x]
+    flags = torch.zeros(1, dtype=torch.int32, device=DEV)
+    tokens = [torch.zeros((20, 6), dtype=torch.int32, device=DEV) for _ in x]
+    logp = [torch.zeros((20, 6), device=DEV) for _ in x]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for v, t, lp, side in zip(x, tokens, logp, sides):
+            with torch.cuda.stream(side):
+                native.sample_launch(v, None, None, p, None, u, t[i], lp[i], flags)
+    torch.cuda.synchronize()
+    for (token, lp, _), t, out in zip(want, tokens, logp):
+        assert bool((t == token).all())
+        assert torch.equal(out.nan_to_num(9.0), lp.nan_to_num(9.0).expand(20, -1))
+    assert int(flags) == 1
+
+
+def test_more_rows_than_places(native):
+    """A hundred thousand short rows, each with its own settings."""
+    m, vocab = 100_003, 37
+    gen = torch.Generator().manual_seed(3)
+    x = (torch.randn((m, vocab), generator=gen) * 3).to(BF16)
+    k = torch.randint(0, 9, (m,), generator=gen, dtype=torch.int32)
+    u = torch.rand(m, generator=gen)
+    tokens, logp, flags = run(native, x.to(DEV), T=0.75, k=k, u=u)
+    w = ((x.double() - x.double().max(1, keepdim=True).values) / 0.75).exp()
+    order = x.double().argsort(dim=1, descending=True, stable=True)
+    rank = torch.empty_like(order).scatter_(1, order, torch.arange(vocab).expand(m, -1).contiguous())
+    w = torch.where((k[:, None] < 1) | (rank < k[:, None]), w, 0.0)
+    cum = w.cumsum(1)
+    target = u.double()[:, None] * cum[:, -1:]
+    want = (cum <= target).sum(1)
+    clear = ((cum - target).abs() > 1e-9).all(1)              # no border so near that 64 bits tell it otherwise
+    assert int(clear.sum()) > 0.999 * m and int(flags) == 0
+    assert torch.equal(tokens.cpu().long()[clear], want[clear])
+    lp = torch.log_softmax(x.double(), 1).gather(1, tokens.cpu().long()[:, None])[:, 0]
+    assert bool(((logp.double().cpu() - lp).abs() <= 2.0 ** -24 * lp.abs() + 1e-12).all())

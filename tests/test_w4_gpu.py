@@ -259,3 +259,31 @@ def test_two_warps_share_a_row_tile(native, group):
         out, flags = run(native, x, bank, n)
         check(out, x, weight)
         assert int(flags) == 0
+
+
+def test_layer_method_on_other_views(native):
+    """No rows, one row of a wider tensor, and a batch whose rows lie apart."""
+    method = importlib.import_module('ornith_b200.method')
+    runtime = importlib.import_module('ornith_b200.runtime')
+    n, k = 96, 128
+    codes, scales, _, weight = make(n, k, 32, False)
+    layer = torch.nn.Module()
+    m = method.W4LinearMethod('layer', group=32)
+    m.create_weights(layer, k, [n], k, n, BF16, device=DEV)
+    layer.w4_codes.weight_loader(layer.w4_codes, codes)
+    layer.w4_scales.weight_loader(layer.w4_scales, scales)
+    m.process_weights_after_loading(layer)
+    rt = runtime.Runtime(['layer'], 8, DEV)
+    m.bind(rt, 0)
+    assert m.apply(layer, torch.empty((0, k), dtype=BF16, device=DEV)).shape == (0, n)
+    assert m.apply(layer, torch.empty((3, 0, k), dtype=BF16, device=DEV)).shape == (3, 0, n)
+    wide = rows(24, 2 * k, BF16)
+    check(m.apply(layer, wide[5, k:])[None], wide[5:6, k:], weight)
+    check(m.apply(layer, wide[:, :k]), wide[:, :k], weight)
+    check(m.apply(layer, wide.view(4, 6, 2 * k).transpose(0, 1)[:, 1:3, k:]).reshape(12, n),
+          wide.view(4, 6, 2 * k).transpose(0, 1)[:, 1:3, k:].reshape(12, k), weight)
+    with pytest.raises(ValueError):
+        m.apply(layer, wide[:, :k].float())
+    with pytest.raises(RuntimeError):
+        m.apply(layer, wide[:, :k], bias=torch.zeros(n, device=DEV))
+    assert rt.check_error_flags() == [0]
