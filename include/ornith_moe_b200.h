@@ -517,8 +517,13 @@ ORNITH_MOE_B200_EXPORT cudaError_t ornith_moe_b200_w4_launch(
  *   order, with sum_{j <= i, j in P} w_j > uniform * mass(P).
  * temperature 0: the largest logit, lowest index.  top_k < 1 or >= vocab,
  * top_p >= 1 and min_p 0 switch their cut off.  logprobs: the model's own
- * x_token - max x - log sum_i exp(x_i - max x).  Weights and their sums are
- * 64-bit fixed point: the token does not depend on the order of summation.
+ * x_token - max x - log sum_i exp(x_i - max x), in 64 bits up to its one
+ * rounding (fp16 and fp32 rows that are cut or have a temperature other than 1
+ * take logits of 2 and more below the largest through fp32 exponentials).
+ * Weights are multiples of 2^-s of the largest, s = min(51, 62 - ceil(log2
+ * vocab)), and their sums exact: the token does not depend on the order of
+ * summation.  Tokens lighter than half of that are drawn by uniform = 0 alone,
+ * which takes the first kept token that has a weight in double precision.
  * -inf logits are never drawn.  A row that cannot be sampled gets token -1 and
  * log probability NaN and raises (sticky) 1: NaN or +inf among its logits,
  * 2: a parameter out of range (temperature outside [0, 1e30], top_p negative,

@@ -7,7 +7,8 @@
 //   token = the first i, in index order, with  sum_{j <= i, j in P} w_j > u * mass(P)
 //
 // T = 0 takes the largest logit (lowest index).  The log probability is the
-// model's own: x_token - max x - log sum_i exp(x_i - max x), over all tokens.
+// model's own: x_token - max x - log sum_i exp(x_i - max x), over all tokens,
+// in 64 bits up to its one rounding (exponentials, counted_partition).
 //
 // Exactness.  The nucleus and the draw compare sums of up to 2^19 weights with
 // the border between two tokens, where fp32 sums would choose another token
@@ -15,7 +16,13 @@
 // 64-bit fixed point, w * 2^s with s = min(51, 62 - ceil(log2 V)): each is
 // computed in double precision (relative error below 2e-13) and rounded once;
 // sums of integers are exact and do not depend on their order, so the same
-// inputs give the same token whatever the launch shape.  The exponential is
+// inputs give the same token whatever the launch shape.  What the rounding costs:
+// a sum is off by half a unit a token at most, by 2^-27 of the largest weight in all
+// for 2^18 tokens (some 2^-36 where the roundings are of either sign), which is how
+// often a random number can find another token than the definition's.  Tokens
+// lighter than 2^-(s+1) weigh nothing, so random numbers between 0 and 2^-24, which
+// fp32 generators do not give, pass them over; for 0 itself tokens are counted down
+// to double precision's smallest weight.  The exponential is
 // table driven (Tang, 1989): 2^-n/256 from a table of 256 values times a Taylor
 // polynomial of degree 3 in the remainder (at most ln 2 / 512, so 2e-13 off).
 // Double-precision steps are what bounds it: tables of 64 and 16 values meet
@@ -39,13 +46,14 @@
 //   - rows that the counts do not hold (many tiny values, a largest logit
 //     outside +-128) search a cut by bins of value.
 //
-// What bounds it.  Not HBM (64 uncut fp32 rows of 248320 take 40.0 us, 1.59
-// TB/s): the small cases wait for some ten steps between the CTAs of a row
-// (17 us for one row), the large ones for the shared-memory counts, a weight's
-// double-precision arithmetic and instruction issue.  Measured: a count of a
-// bf16 row's logits issues at 2.6 instructions a clock; weights take 7.2 clocks
-// for a warp's 32; 256 bf16 rows with a nucleus of many thousand tokens take
-// 111 us (1.15 TB/s) against 729 with a weight for every logit.
+// What bounds it.  Not HBM (64 uncut fp32 rows of 248320 take 44.9 us, 1.42
+// TB/s): the small cases wait for some ten steps between the CTAs of a row (17.6
+// us for one row; the merge of the counts 4.2 of them, an exchange 0.8 to 2.3),
+// the large ones for the shared-memory counts, a weight's double-precision
+// arithmetic and instruction issue: 2.6 instructions a clock over the whole kernel
+// for 256 bf16 rows, and 10.3 clocks for a warp's 32 weights where two CTAs share
+// an SM (13.6 for one alone).  256 bf16 rows with a nucleus of many thousand
+// tokens take 110 us (1.16 TB/s) against 729 with a weight for every logit.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -8,10 +8,10 @@
 // Hadamard rotation, no quantised activations).
 //
 // Arithmetic.  c - z is an integer of at most 4 bits and a sign, exact in bf16
-// and fp16, so every product x * (c - z) is exact in fp32.  Runs of 32 or 64
-// products (never across a group) are summed in the tensor core's fp32
-// accumulator; each run is scaled and added to the row's fp32 sum with one FMA;
-// the only rounding below fp32 is the store in the output's type.
+// and fp16, so every product x * (c - z) is exact in fp32.  A group's products
+// (32 to 256, 2 to 16 chained steps) are summed in the tensor core's fp32
+// accumulator; each group's sum is scaled and added to the row's fp32 sum with one
+// FMA; the only rounding below fp32 is the store in the output's type.
 //
 // Layout.  A tile is 16 rows of N times 64 values of K = 512 bytes, lane
 // l = 4r + t holding 16 of them as four words, one per mma.m16n8k16 step, in
@@ -25,13 +25,17 @@
 //
 // What bounds it: the stream of the codes, N*K/2 bytes.  One warp reads a tile
 // with one 16-byte load per lane, two or four tiles ahead in registers.  248320
-// x 2048 with groups of 128 for one bf16 row: 55.3 us, 262 MB at 4.74 TB/s (0.72
-// of a copy's measured 6.55); groups of 64 with zero points, 8 rows: 67.4 us,
-// 4.18 TB/s (0.64).  There the warps issue 2.5 instructions a clock, most of
-// them to take a nibble out and centre it, so loads come no faster; a ring of
-// asynchronous copies in a persistent kernel took 71 and 90 us.  12288 x 2048
-// takes 5.0 us for one row and 7.0 for 16, 2048 x 512 2.4: the launch, and one
-// latency of memory for the codes and one for the join.
+// x 2048 with groups of 128 for one bf16 row: 55.8 us, 263 MB at 4.72 TB/s (0.72
+// of a copy's measured 6.55); groups of 64 with zero points, 8 rows: 69.0 us,
+// 4.09 TB/s (0.62).  There the warps issue 2.3 and 2.5 instructions a clock, most
+// of them to take a nibble out and centre it (the integer units are busy for 57 %
+// of the time), so loads come no faster; a ring of asynchronous copies in a
+// persistent kernel took 71 and 90 us.  12288 x 2048 takes 5.0 us for one row and
+// 8.6 for 16 with groups of 32, 2048 x 512 2.1: the launch, and one latency of
+// memory for the codes and one for the join.
+//
+// For more than 16 rows a caller has to come again and the codes are streamed
+// again: it is a kernel for decode steps.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>

@@ -752,6 +752,10 @@ def w4_pack_shapes(n, k, group):
 def w4_pack(codes, scales, zeros=None):
     """Lay a 4-bit weight out for w4_launch, once when it is loaded.
 
+    Checkpoints differ in how they pack: int32 codes are viewed as uint32; zero
+    points that come eight to a word have to be unpacked to a byte each, and
+    codes packed along N or in another order of nibbles brought into this one.
+
     codes uint32 [N, K/8] (value 8j + d of a row in bits 4d of its word j),
     scales bf16 or fp16 [N, K/group], zeros uint8 [N, K/group] in 0..15 or None
     for 8 everywhere.  Returns (tiles, scales, zeros) on the same device.
@@ -793,6 +797,7 @@ def _launch_on(index, fn, *args):
 def w4_launch(x, tiles, scales, zeros, out, flags, n, k):
     """out [M, n] (x's type or fp32) = x [M <= 16, k] (bf16 or fp16) times the
     transposed weight [n, k] that w4_pack laid out as (tiles, scales, zeros).
+    More rows take one call for every 16, each of which streams the weight.
     x may have rows further apart than k (a multiple of 8 values, rows on 16
     bytes).  flags receives the dense bits 4 (non-finite result) and 8
     (non-finite stored value)."""
@@ -861,10 +866,19 @@ def sample_launch(logits, temperature, top_k, top_p, min_p, uniform, tokens, log
     and min_p 0 switch their cut off for a row.  logprobs fp32 [M] or None: the
     model's own log probability of the token, over all tokens at temperature 1.
 
+    Weights are multiples of 2^-s of the largest, s = min(51, 62 - ceil(log2
+    V)), and their sums exact, so the token depends neither on the order of
+    summation nor on the rows beside it.  uniform is meant to come from an fp32
+    generator (0 or at least 2^-24): between the two, tokens lighter than half
+    of that unit are passed over; 0 takes the first kept token that has a weight
+    in double precision.
+
     A row that cannot be sampled gets token -1 and log probability NaN and
     raises a bit of flags: 1 NaN or +inf among its logits, 2 a parameter out of
     range (temperature outside [0, 1e30], negative top_p, min_p outside [0, 1],
-    uniform outside [0, 1), any NaN), 4 every logit -inf."""
+    uniform outside [0, 1), any NaN), 4 every logit -inf, 128 a defect of the
+    kernel (none is known).  The word is best a caller's own: in a slot that a
+    WorkerStepLifecycle checks, one request's bad parameter ends the worker."""
     index, shape = logits.get_device(), logits.shape
     if (len(shape) != 2 or logits.dtype not in _TYPES or index < 0 or not 0 < shape[1] <= SAMPLE_MAX_VOCAB
             or (shape[1] > 1 and logits.stride(1) != 1)):
